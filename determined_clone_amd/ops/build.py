@@ -47,6 +47,10 @@ def _common_flags(abi: int) -> List[str]:
             "-D__HIP_PLATFORM_AMD__=1", "-Wno-unused-result", "-Wno-deprecated-declarations"]
 
 
+# No packed fp32 arithmetic (v_pk_add / mul / fma_f32, which -O3 forms from ordinary float code): some
+# of its forms have given wrong results on gfx950 now and then, with no error.
+_HIP_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 # per-source extra flags. attention.hip: no SLP vectorizer -- it packs the softmax-gradient
 # subtract/multiply pairs into v_pk_add_f32 / v_pk_mul_f32, which cost ~24 extra cycles each beside
 # MFMAs on gfx950 (cdna guide: packed f32 VALU is an anti-lever in MFMA loops)
@@ -57,7 +61,7 @@ def source_hash() -> str:
     """sha256 over the names and bytes of every ``csrc/`` source and header plus the target arch and
     per-file flags: the identity of a correct ``_C.so`` for this tree."""
     h = hashlib.sha256()
-    h.update(f"arch={ARCH};flags={sorted(_FILE_FLAGS.items())}".encode())
+    h.update(f"arch={ARCH};flags={_HIP_FLAGS + sorted(_FILE_FLAGS.items())}".encode())
     for f in sorted(CSRC.iterdir()):
         if f.suffix in (".hip", ".cpp", ".h"):
             h.update(f.name.encode() + b"\0" + f.read_bytes() + b"\0")
@@ -101,7 +105,7 @@ def build(force: bool = False, verbose: bool = False, jobs: int = 0, defines: Se
         obj = BUILD_ / (src.stem + ".hip.o")
         objs.append(obj)
         cmd = [_hipcc(), "-c", str(src), "-o", str(obj), f"--offload-arch={ARCH}",
-               "-munsafe-fp-atomics", f"-I{CSRC}"] + _common_flags(abi) + _FILE_FLAGS.get(src.stem, []) + dflags
+               "-munsafe-fp-atomics", f"-I{CSRC}"] + _common_flags(abi) + _HIP_FLAGS + _FILE_FLAGS.get(src.stem, []) + dflags
         key = _obj_key(src, headers, cmd)
         if force or _stale(obj, key):
             jobs_list.append((cmd, key))
