@@ -581,6 +581,7 @@ void scale_(const Tensor& x, double s, const OptT& dev_scale) {
 void register_transformer_ops(pybind11::module& m);
 void register_conv_ops(pybind11::module& m);
 void register_groupnorm_ops(pybind11::module& m);
+void register_embedding_ops(pybind11::module& m);
 void register_lt_ops(pybind11::module& m);
 
 extern "C" const char dca_source_hash[];  // ops/build.py: sha256 of the csrc/ tree
@@ -626,5 +627,6 @@ PYBIND11_MODULE(_C, m) {
   register_transformer_ops(m);
   register_conv_ops(m);
   register_groupnorm_ops(m);
+  register_embedding_ops(m);
   register_lt_ops(m);
 }

@@ -1,0 +1,127 @@
+"""Token embedding for language models: table lookup with scaling, learned positions added in the
+same pass, vocabulary shards, and the table gradients.
+
+GPU path: ``ops/csrc/embedding.hip``; CPU path (and oracle of the GPU tests): plain PyTorch. The
+reference's GPT-NeoX example gets these from Megatron's ``VocabParallelEmbedding`` and
+``torch.nn.Embedding`` (reference: examples/deepspeed/gpt_neox/gpt2_trial.py).
+
+The token gradient sums the rows of each token in token order (ids sorted on the GPU, no float
+atomics), so it does not change from run to run. With a persistent ``.grad`` (``ops._grad``) only
+the rows of tokens that occur are touched, added in place; otherwise a dense gradient is returned.
+"""
+from typing import Optional
+
+import torch
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from determined_clone_amd.ops import _ext, _grad
+
+_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def reference_embedding(idx, weight, pos_weight=None, positions=None, scale=1.0, vocab_start=None):
+    """The same operator in plain PyTorch (fp32 or wider arithmetic, rounded once)."""
+    local = idx.long() - (vocab_start or 0)
+    wide = torch.promote_types(weight.dtype, torch.float32)
+    if vocab_start is None:
+        out = F.embedding(local, weight).to(wide) * scale
+    else:
+        outside = (local < 0) | (local >= weight.shape[0])
+        out = F.embedding(local.masked_fill(outside, 0), weight).to(wide) * scale
+        out = out.masked_fill(outside.unsqueeze(-1), 0)
+    if pos_weight is not None:
+        if positions is None:
+            out = out + pos_weight[:idx.shape[-1]].to(wide)
+        else:
+            out = out + F.embedding(positions.long(), pos_weight).to(wide)
+    return out.to(weight.dtype)
+
+
+def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, idx, weight, pos_weight, positions, scale, vocab_start):
+        ctx.save_for_backward(idx, positions)
+        ctx.params = (weight, pos_weight)
+        ctx.scale, ctx.start = scale, vocab_start or 0
+        return _ext.load().embed_fwd(idx, _rows(weight.detach()),
+                                     None if pos_weight is None else _rows(pos_weight.detach()),
+                                     positions, scale, ctx.start, vocab_start is not None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        C = _ext.load()
+        idx, positions = ctx.saved_tensors
+        weight, pos_weight = ctx.params
+        dw = dp = None
+        dy = dy.contiguous()
+        if ctx.needs_input_grad[1]:
+            acc = _grad.target(weight)
+            dw = C.embed_grad(dy, idx, weight.shape[0], ctx.scale, ctx.start, acc)
+            dw = None if acc is not None else dw
+        if ctx.needs_input_grad[2]:
+            acc = _grad.target(pos_weight)
+            if positions is None:
+                dp = C.embed_pos_grad(dy, pos_weight.shape[0], acc)
+            else:
+                dp = C.embed_grad(dy, positions, pos_weight.shape[0], 1.0, 0, acc)
+            dp = None if acc is not None else dp
+        return None, dw, dp, None, None, None
+
+
+def _check_index(t: torch.Tensor, what: str) -> None:
+    if t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"embedding: {what} must be int32 or int64, got {t.dtype}")
+
+
+def embedding(idx: torch.Tensor, weight: torch.Tensor, pos_weight: Optional[torch.Tensor] = None,
+              positions: Optional[torch.Tensor] = None, scale: float = 1.0,
+              vocab_start: Optional[int] = None) -> torch.Tensor:
+    """``scale * weight[idx] (+ pos_weight[positions])`` for ``idx`` [...] and ``weight`` [V, E] ->
+    [..., E] in the table's dtype, computed in fp32 and rounded once.
+
+    ``pos_weight`` [P, E] adds learned positions: row ``s`` to the tokens at index ``s`` of the last
+    dim of ``idx`` (at most P of them), or row ``positions[...]`` when ``positions`` (int32 / int64,
+    broadcastable to ``idx``) is given: packed documents, generation from an offset.
+
+    ``vocab_start`` makes ``weight`` a shard of a larger vocabulary, rows ``vocab_start`` and up: ids
+    outside it look up zeros and have no gradient (sum the shards' outputs with an all-reduce).
+    Without it every id has to lie in [0, V), and every position in [0, P): the CPU path raises
+    ``IndexError`` for others, the GPU path, which does not wait for the values, returns NaN rows
+    for them and gives them no gradient in the table that they miss."""
+    _check_index(idx, "idx")
+    if weight.dim() != 2 or not weight.is_floating_point():
+        raise ValueError("embedding: weight must be a floating-point [V, E] table")
+    if idx.device != weight.device:
+        raise ValueError(f"embedding: idx on {idx.device}, weight on {weight.device}")
+    if positions is not None and pos_weight is None:
+        raise ValueError("embedding: positions without pos_weight")
+    if pos_weight is not None:
+        if vocab_start is not None:
+            raise ValueError("embedding: add positions after the vocabulary shards are summed")
+        if pos_weight.dim() != 2 or pos_weight.shape[1] != weight.shape[1] or \
+                pos_weight.dtype != weight.dtype or pos_weight.device != weight.device:
+            raise ValueError("embedding: pos_weight must be [P, E] like weight (width, dtype, device)")
+        if positions is not None:
+            _check_index(positions, "positions")
+            if positions.device != weight.device:
+                raise ValueError(f"embedding: positions on {positions.device}, weight on {weight.device}")
+            positions = positions.expand(idx.shape)  # raises for shapes that do not broadcast
+        elif idx.dim() == 0:
+            raise ValueError("embedding: a single id needs its position")
+        elif idx.shape[-1] > pos_weight.shape[0]:
+            raise ValueError(f"embedding: {idx.shape[-1]} tokens, {pos_weight.shape[0]} positions")
+    if not weight.is_cuda:
+        return reference_embedding(idx, weight, pos_weight, positions, scale, vocab_start)
+    if weight.dtype not in _DTYPES:
+        raise ValueError(f"embedding: GPU path needs bf16, fp16 or fp32 tables, got {weight.dtype}")
+    return _Embedding.apply(idx.contiguous(), weight, pos_weight,
+                            None if positions is None else positions.contiguous(), float(scale), vocab_start)
+
+
+__all__ = ["embedding", "reference_embedding"]

@@ -1,0 +1,84 @@
+"""Embedding (lookup, scaling, positions, vocabulary shards) on the CPU: results, gradients against
+finite differences, refusals."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+from determined_clone_amd.ops.embedding import embedding
+
+
+def test_matches_nn_embedding():
+    g = torch.Generator().manual_seed(0)
+    w, p = torch.randn(50, 12, generator=g), torch.randn(9, 12, generator=g)
+    idx = torch.randint(0, 50, (3, 7), generator=g)
+    torch.testing.assert_close(embedding(idx, w), F.embedding(idx, w), rtol=0, atol=0)
+    torch.testing.assert_close(embedding(idx, w, p), F.embedding(idx, w) + p[:7], rtol=0, atol=0)
+    pos = torch.randint(0, 9, (3, 7), generator=g)
+    torch.testing.assert_close(embedding(idx.int(), w, p, positions=pos, scale=2.0),
+                               2 * F.embedding(idx, w) + p[pos], rtol=0, atol=0)
+    # one position row for all sequences broadcasts
+    torch.testing.assert_close(embedding(idx, w, p, positions=pos[0]), F.embedding(idx, w) + p[pos[0]],
+                               rtol=0, atol=0)
+
+
+def test_low_precision_rounds_once():
+    # 1 + 2^-8 is not a bf16 number, but the fp32 sum is: rounding w * scale first would lose it
+    w = torch.full((1, 1), 1.0078125).bfloat16()  # 1 + 2^-7
+    p = torch.full((1, 1), -1.0).bfloat16()
+    out = embedding(torch.zeros(1, 1, dtype=torch.long), w, p, scale=1.00390625)  # 1 + 2^-8
+    want = 1.0078125 * 1.00390625 - 1.0
+    assert abs(out.item() - want) <= abs(want) * 2.0 ** -8
+
+
+def test_shards_sum_to_the_whole():
+    g = torch.Generator().manual_seed(1)
+    w = torch.randn(40, 6, generator=g)
+    idx = torch.randint(0, 40, (5, 4), generator=g)
+    parts = [embedding(idx, w[s:s + 10], vocab_start=s, scale=3.0) for s in range(0, 40, 10)]
+    torch.testing.assert_close(sum(parts), 3 * F.embedding(idx, w), rtol=0, atol=0)
+
+
+def test_gradients_against_differences():
+    g = torch.Generator().manual_seed(2)
+    w = torch.randn(5, 3, generator=g, dtype=torch.float64).requires_grad_(True)
+    p = torch.randn(4, 3, generator=g, dtype=torch.float64).requires_grad_(True)
+    idx = torch.tensor([[0, 4, 4], [2, 0, 4]])
+    pos = torch.tensor([[3, 3, 0], [1, 0, 0]])
+    assert torch.autograd.gradcheck(lambda a, b: embedding(idx, a, b, scale=1.5), (w, p))
+    assert torch.autograd.gradcheck(lambda a, b: embedding(idx, a, b, positions=pos), (w, p))
+    assert torch.autograd.gradcheck(lambda a: embedding(idx, a[1:4], vocab_start=1), (w,))
+
+
+def test_empty_and_single():
+    w = torch.randn(5, 4)
+    assert embedding(torch.zeros(2, 0, dtype=torch.long), w).shape == (2, 0, 4)
+    assert embedding(torch.tensor(3), w).shape == (4,)
+    torch.testing.assert_close(embedding(torch.tensor(3), w, w, positions=torch.tensor(1)), w[3] + w[1])
+
+
+def test_refusals():
+    w, idx = torch.randn(5, 4), torch.zeros(2, 3, dtype=torch.long)
+    with pytest.raises(ValueError, match="int32 or int64"):
+        embedding(idx.float(), w)
+    with pytest.raises(ValueError, match="int32 or int64"):
+        embedding(idx, w, w, positions=idx.to(torch.int16))
+    with pytest.raises(ValueError, match="positions without"):
+        embedding(idx, w, positions=idx)
+    with pytest.raises(ValueError, match="pos_weight must be"):
+        embedding(idx, w, torch.randn(5, 3))
+    with pytest.raises(ValueError, match="pos_weight must be"):
+        embedding(idx, w, w.double())
+    with pytest.raises(ValueError, match="tokens"):
+        embedding(idx, w, w[:2])
+    with pytest.raises(ValueError, match="single id"):
+        embedding(idx[0, 0], w, w)
+    with pytest.raises(ValueError, match="shards"):
+        embedding(idx, w, w, vocab_start=0)
+    with pytest.raises(ValueError, match="table"):
+        embedding(idx, w[0])
+    with pytest.raises(RuntimeError):
+        embedding(idx, w, w, positions=torch.zeros(2, dtype=torch.long))
+    with pytest.raises(IndexError):
+        embedding(idx + 5, w)
+    with pytest.raises(IndexError):
+        embedding(idx, w, w, positions=idx - 1)
