@@ -583,6 +583,7 @@ void register_conv_ops(pybind11::module& m);
 void register_groupnorm_ops(pybind11::module& m);
 void register_embedding_ops(pybind11::module& m);
 void register_qk_norm_ops(pybind11::module& m);
+void register_grad_norm_ops(pybind11::module& m);
 void register_lt_ops(pybind11::module& m);
 
 extern "C" const char dca_source_hash[];  // ops/build.py: sha256 of the csrc/ tree
@@ -630,5 +631,6 @@ PYBIND11_MODULE(_C, m) {
   register_groupnorm_ops(m);
   register_embedding_ops(m);
   register_qk_norm_ops(m);
+  register_grad_norm_ops(m);
   register_lt_ops(m);
 }

@@ -16,7 +16,7 @@ DeepSpeed FusedAdam/FusedLamb) and `PyTorchTrialContext.step_optimizer` clipping
 (`harness/determined/pytorch/_pytorch_context.py:827`).
 """
 import math
-from typing import Any, Callable, Dict, List, Optional
+from typing import Any, Callable, Dict, Iterable, List, Optional
 
 import torch
 
@@ -516,6 +516,62 @@ class DeviceGradScaler:
         self.growth_factor = sd.get("growth_factor", self.growth_factor)
         self.backoff_factor = sd.get("backoff_factor", self.backoff_factor)
         self.growth_interval = sd.get("growth_interval", self.growth_interval)
+
+
+# ------------------------------------------------------------------------- separate gradients
+_NORM_KINDS = {2.0: 0, 1.0: 1, math.inf: 2}  # NormKind in ops/csrc/grad_norm_api.h
+
+
+def _list_kernel(grads: List[torch.Tensor], norm_type: float, max_norm: Optional[float]) -> Optional[torch.Tensor]:
+    """The total norm by the multi-tensor kernels (and clipping to ``max_norm``), or None where they
+    do not apply: see :func:`clip_grad_norm_`."""
+    kind = _NORM_KINDS.get(norm_type)
+    if kind is None or not grads or not grads[0].is_cuda:
+        return None
+    _grad.join()  # weight gradients still running on the side stream
+    return _ext.load().grad_list_norm(grads, kind, max_norm)
+
+
+@torch.no_grad()
+def grad_norm(grads: Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
+    """The norm of all ``grads`` together (2, 1 or ``inf``; others as in
+    ``torch.nn.utils.get_total_norm``) as an fp32 scalar on their device, without synchronisation:
+    one read of every tensor, sums in 64 bits, the same bits on every run."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    norm_type = float(norm_type)
+    total = _list_kernel(grads, norm_type, None)
+    return torch.nn.utils.get_total_norm(grads, norm_type).float() if total is None else total
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: Any, max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """``torch.nn.utils.clip_grad_norm_`` for separate gradient tensors on one GPU: scales the
+    ``.grad`` of ``parameters`` (a tensor or an iterable) in place so that their norm together is at
+    most ``max_norm``, and returns the norm before that, an fp32 scalar on their device.
+
+    bf16, fp16 and fp32 gradients in any mix and number go through the multi-tensor kernels: the sums
+    are held in 64 bits, the coefficient in fp32, and gradients within the limit are not rewritten.
+    CPU, float64, sparse, strided (not dense), overlapping or multi-device gradients and other norms
+    than 2, 1 and ``inf`` go to ``torch.nn.utils.clip_grad_norm_``. Nothing synchronises unless
+    ``error_if_nonfinite``."""
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in params if p.grad is not None]
+    max_norm, norm_type = float(max_norm), float(norm_type)
+    # a norm that may be refused is looked at before anything is scaled
+    total = _list_kernel(grads, norm_type, None if error_if_nonfinite else max_norm)
+    if total is None:
+        # tensors that share memory one after the other: a multi-tensor pass would race on them
+        foreach = False if grads and grads[0].is_cuda and _ext.load().grad_list_overlaps(grads) else None
+        return torch.nn.utils.clip_grad_norm_(params, max_norm, norm_type, error_if_nonfinite, foreach)
+    if error_if_nonfinite:
+        if not torch.isfinite(total):
+            raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is "
+                               "non-finite, so it cannot be clipped. Set `error_if_nonfinite=False` to "
+                               "scale the gradients by the non-finite norm anyway")
+        if _ext.load().grad_list_clip(grads, total, max_norm) is None:  # they share memory
+            return torch.nn.utils.clip_grad_norm_(params, max_norm, norm_type, True, False)
+    return total
 
 
 def fuse_optimizer(opt: torch.optim.Optimizer) -> Optional[FusedOptimizerBase]:

@@ -34,14 +34,14 @@ logger = logging.getLogger("determined_clone_amd.pytorch")
 
 class ClipGradNorm:
     """Marker clip function recognised by ``step_optimizer``: with a fused optimizer the global
-    L2 norm + scaling run on the device inside the optimizer step; otherwise it falls back to
-    ``torch.nn.utils.clip_grad_norm_``."""
+    L2 norm + scaling run on the device inside the optimizer step; otherwise they run over the
+    separate gradients (``ops.optim.clip_grad_norm_``)."""
 
     def __init__(self, max_norm: float) -> None:
         self.max_norm = float(max_norm)
 
     def __call__(self, params: Any) -> Any:
-        return torch.nn.utils.clip_grad_norm_(list(params), self.max_norm)
+        return fused_optim.clip_grad_norm_(params, self.max_norm)
 
 
 def clip_grad_norm(max_norm: float) -> ClipGradNorm:
