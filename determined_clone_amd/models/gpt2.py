@@ -13,8 +13,11 @@ MI355X layout decisions:
 * MLP up-projection runs without bias in hipBLASLt and the bias + tanh-GELU are one fused kernel;
 * GEMM weights are bf16; LayerNorm affine parameters stay fp32 (they are read by the LN kernels as
   fp32 and keep their own flat fp32 buffer in the optimizer);
+* token and learned-position rows are looked up and added in one pass, and their gradients are
+  added straight into the persistent ``.grad`` tables (``ops.embedding``);
 * position encoding: learned absolute (GPT-2) or rotary on the first ``rotary_pct`` of each head
-  (GPT-NeoX, rotate-half convention, fused RoPE kernel).
+  (GPT-NeoX, rotate-half convention, fused RoPE kernel); ``qk_norm`` puts an RMS norm on every query
+  and key head, in the same pass as the rotation (``ops.qk_norm``).
 """
 import math
 from dataclasses import dataclass, field
@@ -25,6 +28,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from determined_clone_amd.ops import transformer as T
+from determined_clone_amd.ops.embedding import embedding
+from determined_clone_amd.ops.qk_norm import qk_norm_attention_qkvpacked
 
 
 @dataclass
@@ -43,6 +48,7 @@ class GPTConfig:
     dropout: float = 0.0
     init_std: float = 0.02
     pad_vocab_multiple: int = 128
+    qk_norm: bool = False  # RMS norm of every query and key head (one weight per feature, fp32)
     extra: Dict = field(default_factory=dict)
 
     @property
@@ -87,10 +93,29 @@ class FusedLayerNorm(nn.Module):
         return T.layer_norm(x, self.weight, self.bias, self.eps, residual=residual)
 
 
+class TokenEmbedding(nn.Embedding):
+    """Token table; ``forward(idx, pos_weight)`` adds the rows of a learned-position table."""
+
+    def forward(self, idx: torch.Tensor, pos_weight: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return embedding(idx, self.weight, pos_weight)
+
+
+class HeadNorm(nn.Module):
+    """Weight of the RMS norm of the query or key heads, applied by the attention op."""
+
+    keep_fp32 = True
+
+    def __init__(self, head_dim: int) -> None:
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(head_dim))
+
+
 class Attention(nn.Module):
     def __init__(self, cfg: GPTConfig) -> None:
         super().__init__()
         self.cfg = cfg
+        self.q_norm = HeadNorm(cfg.head_dim) if cfg.qk_norm else None
+        self.k_norm = HeadNorm(cfg.head_dim) if cfg.qk_norm else None
         E = cfg.d_model
         self.qkv = nn.Linear(E, 3 * E)
         self.proj = nn.Linear(E, E)
@@ -105,7 +130,11 @@ class Attention(nn.Module):
         B, S, E = x.shape
         H, D = self.cfg.n_head, self.cfg.head_dim
         qkv = T.linear(x, self.qkv.weight, self.qkv.bias).view(B, S, 3, H, D)
-        if self.rot:
+        if self.q_norm is not None:
+            cos, sin = rope_cache if self.rot else (None, None)
+            o = qk_norm_attention_qkvpacked(qkv, self.q_norm.weight, self.k_norm.weight, cos, sin,
+                                            rot_dim=self.rot, eps=self.cfg.ln_eps, causal=True)
+        elif self.rot:
             q, k, v = qkv.unbind(2)
             cos, sin = rope_cache
             q = T.rope(q, cos, sin, self.rot)
@@ -159,7 +188,7 @@ class GPT(nn.Module):
         super().__init__()
         self.cfg = cfg
         V, E = cfg.padded_vocab, cfg.d_model
-        self.wte = nn.Embedding(V, E)
+        self.wte = TokenEmbedding(V, E)
         self.wpe = nn.Embedding(cfg.max_seq_len, E) if cfg.pos_emb == "learned" else None
         self.blocks = nn.ModuleList([Block(cfg) for _ in range(cfg.n_layer)])
         self.ln_f = FusedLayerNorm(E, cfg.ln_eps)
@@ -204,10 +233,7 @@ class GPT(nn.Module):
         return float(dense + attn)
 
     def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None):
-        B, S = idx.shape
-        x = self.wte(idx)
-        if self.wpe is not None:
-            x = x + self.wpe.weight[:S].unsqueeze(0)
+        x = self.wte(idx, None if self.wpe is None else self.wpe.weight)
         rope = (self.rope_cos, self.rope_sin) if self.cfg.pos_emb == "rotary" else None
         resid, delta = x, None
         for blk in self.blocks:
@@ -241,15 +267,12 @@ class EmbeddingPipe(nn.Module):
     def __init__(self, cfg: GPTConfig) -> None:
         super().__init__()
         self.cfg = cfg
-        self.wte = nn.Embedding(cfg.padded_vocab, cfg.d_model)
+        self.wte = TokenEmbedding(cfg.padded_vocab, cfg.d_model)
         self.wpe = nn.Embedding(cfg.max_seq_len, cfg.d_model) if cfg.pos_emb == "learned" else None
         _init_like_gpt(self, cfg)
 
     def forward(self, idx: torch.Tensor) -> torch.Tensor:
-        x = self.wte(idx)
-        if self.wpe is not None:
-            x = x + self.wpe.weight[:idx.shape[1]].unsqueeze(0)
-        return x
+        return self.wte(idx, None if self.wpe is None else self.wpe.weight)
 
 
 class BlockPipe(Block):

@@ -12,8 +12,8 @@ The reference's GPT-NeoX trial trains with ``model_parallel_size: 2``
   down-projection row-parallel -> one all-reduce per MLP;
 * token embedding and the tied LM head are vocab-parallel; the loss is the vocab-parallel
   cross-entropy, so the [tokens, vocab] logits are never gathered;
-* LayerNorms, position embeddings and row-parallel biases are replicated (identical gradients on
-  every TP rank; :func:`~determined_clone_amd.parallel.tensor.tp_norm_setup` counts them once).
+* LayerNorms, position embeddings, row-parallel biases and the query / key norms' weights (whose
+  gradient is summed over the ranks' heads) are replicated (identical gradients on every TP rank; :func:`~determined_clone_amd.parallel.tensor.tp_norm_setup` counts them once).
 
 ``TPGPT.load_from(full)`` copies a dense model's weights into the shards (parity tests, and
 converting dense checkpoints); ``full_state_dict()`` gathers them back.
@@ -25,8 +25,9 @@ import torch.distributed as dist
 import torch.nn as nn
 import torch.nn.functional as F
 
-from determined_clone_amd.models.gpt2 import GPT, FusedLayerNorm, GPTConfig, _init_like_gpt
+from determined_clone_amd.models.gpt2 import GPT, FusedLayerNorm, GPTConfig, HeadNorm, _init_like_gpt
 from determined_clone_amd.ops import transformer as T
+from determined_clone_amd.ops.qk_norm import qk_norm_attention_qkvpacked
 from determined_clone_amd.parallel import tensor as tp
 
 
@@ -41,6 +42,8 @@ class TPAttention(nn.Module):
         E = cfg.d_model
         self.qkv = tp.ColumnParallelLinear(E, 3 * E, group)
         self.proj = tp.RowParallelLinear(E, E, group)
+        self.q_norm = HeadNorm(cfg.head_dim) if cfg.qk_norm else None
+        self.k_norm = HeadNorm(cfg.head_dim) if cfg.qk_norm else None
         self.rot = 0
         if cfg.pos_emb == "rotary":
             rot = int(cfg.head_dim * cfg.rotary_pct)
@@ -57,7 +60,12 @@ class TPAttention(nn.Module):
         B, S, _ = x.shape
         H, D = self.local_heads, self.cfg.head_dim
         qkv = self.qkv(x).view(B, S, 3, H, D)
-        if self.rot:
+        if self.q_norm is not None:
+            cos, sin = rope_cache if self.rot else (None, None)
+            wq, wk = (tp.copy_to_tp(n.weight, self.group) for n in (self.q_norm, self.k_norm))
+            o = qk_norm_attention_qkvpacked(qkv, wq, wk, cos, sin, rot_dim=self.rot, eps=self.cfg.ln_eps,
+                                            causal=True)
+        elif self.rot:
             q, k, v = qkv.unbind(2)
             cos, sin = rope_cache
             o = T.flash_attention(T.rope(q, cos, sin, self.rot), T.rope(k, cos, sin, self.rot), v,
@@ -67,6 +75,12 @@ class TPAttention(nn.Module):
         if self.cfg.dropout and self.training:
             o = F.dropout(o, self.cfg.dropout)
         return self.proj(o.reshape(B, S, H * D))
+
+
+def _load_head_norms(attn: TPAttention, full: nn.Module) -> None:
+    if attn.q_norm is not None:
+        attn.q_norm.load_state_dict(full.q_norm.state_dict())
+        attn.k_norm.load_state_dict(full.k_norm.state_dict())
 
 
 class TPMLP(nn.Module):
@@ -157,6 +171,7 @@ class TPGPT(nn.Module):
             b.attn.proj.load_full(fb.attn.proj.weight, fb.attn.proj.bias)
             b.mlp.fc.load_full(fb.mlp.fc.weight, fb.mlp.fc.bias)
             b.mlp.proj.load_full(fb.mlp.proj.weight, fb.mlp.proj.bias)
+            _load_head_norms(b.attn, fb.attn)
         return self
 
     def full_state_dict(self) -> Dict[str, torch.Tensor]:
@@ -186,6 +201,8 @@ class TPGPT(nn.Module):
             for name, t in (("weight", b.attn.qkv.weight), ("bias", b.attn.qkv.bias)):
                 g = gather(t, 0).reshape(n, 3, Hl * D, *t.shape[1:])
                 out[p + f"attn.qkv.{name}"] = g.transpose(0, 1).reshape(3 * E, *t.shape[1:])
+            for norm in ("q_norm", "k_norm") if self.cfg.qk_norm else ():
+                out[p + f"attn.{norm}.weight"] = getattr(b.attn, norm).weight.detach().clone()
             out[p + "attn.proj.weight"] = gather(b.attn.proj.weight, 1)
             out[p + "attn.proj.bias"] = b.attn.proj.bias.detach().clone()
             out[p + "mlp.fc.weight"] = gather(b.mlp.fc.weight, 0)
@@ -303,5 +320,6 @@ def load_pipeline_from(pipe_module: nn.Module, full: GPT) -> None:
             mod.attn.proj.load_full(fb.attn.proj.weight, fb.attn.proj.bias)
             mod.mlp.fc.load_full(fb.mlp.fc.weight, fb.mlp.fc.bias)
             mod.mlp.proj.load_full(fb.mlp.proj.weight, fb.mlp.proj.bias)
+            _load_head_norms(mod.attn, fb.attn)
         elif idx == L + 1:
             mod.ln_f.load_state_dict(full.ln_f.state_dict())

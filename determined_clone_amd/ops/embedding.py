@@ -116,10 +116,8 @@ def embedding(idx: torch.Tensor, weight: torch.Tensor, pos_weight: Optional[torc
             raise ValueError("embedding: a single id needs its position")
         elif idx.shape[-1] > pos_weight.shape[0]:
             raise ValueError(f"embedding: {idx.shape[-1]} tokens, {pos_weight.shape[0]} positions")
-    if not weight.is_cuda:
+    if not weight.is_cuda or weight.dtype not in _DTYPES:  # float64 tables: plain PyTorch
         return reference_embedding(idx, weight, pos_weight, positions, scale, vocab_start)
-    if weight.dtype not in _DTYPES:
-        raise ValueError(f"embedding: GPU path needs bf16, fp16 or fp32 tables, got {weight.dtype}")
     return _Embedding.apply(idx.contiguous(), weight, pos_weight,
                             None if positions is None else positions.contiguous(), float(scale), vocab_start)
 

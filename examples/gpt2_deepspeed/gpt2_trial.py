@@ -9,6 +9,8 @@ MI355X engine: ZeRO-1/2 over RCCL, fused HIP AdamW, MFMA flash attention, fused 
 split, gradients averaged over the data-parallel group only; both together (``pipe_tp.yaml``) is
 the reference's ``zero1.yaml`` layout: a pipeline of tensor-parallel stages.
 
+``hyperparameters.qk_norm: true`` puts an RMS norm on every query and key head.
+
 The DeepSpeed JSON config is ``ds_config.json`` overlaid with ``hyperparameters.overwrite_deepspeed_args``
 (same convention as the reference's ``overwrite_deepspeed_config``). Synthetic token data."""
 import json
@@ -39,7 +41,8 @@ class GPT2Trial(det_ds.DeepSpeedTrial):
         self.context = context
         hp = context.get_hparams()
         self.seq = int(hp.get("seq_len", 1024))
-        cfg = gpt2.config_for(hp.get("model", "gpt2-medium"), max_seq_len=self.seq)
+        cfg = gpt2.config_for(hp.get("model", "gpt2-medium"), max_seq_len=self.seq,
+                              qk_norm=bool(hp.get("qk_norm", False)))
         base = json.load(open(os.path.join(os.path.dirname(os.path.abspath(__file__)), "ds_config.json")))
         ds_config = det_ds.overwrite_deepspeed_config(base, hp.get("overwrite_deepspeed_args", {}))
         self.pipe = int(hp.get("pipe_parallel_size", 0))

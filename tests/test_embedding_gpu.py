@@ -235,13 +235,16 @@ def test_on_a_side_stream_and_two_calls_at_once():
     assert all(torch.equal(t, want) for t in got)
 
 
+def test_float64_tables_take_plain_torch():
+    idx, w, p, _ = _inputs(2, 6, 30, 16, torch.float32, p=8)
+    torch.testing.assert_close(embedding(idx, w.double(), p.double(), scale=2.0), 2 * w.double()[idx] + p.double()[:6])
+
+
 def test_refusals():
     w = torch.randn(5, 4, device="cuda")
     idx = torch.zeros(2, 3, dtype=torch.long, device="cuda")
     with pytest.raises(ValueError, match="idx on"):
         embedding(idx.cpu(), w)
-    with pytest.raises(ValueError, match="GPU path"):
-        embedding(idx, w.double())
     with pytest.raises(ValueError, match="positions on"):
         embedding(idx, w, w, positions=idx.cpu())
     with pytest.raises(RuntimeError, match="must be"):

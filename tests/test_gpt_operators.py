@@ -1,0 +1,169 @@
+"""GPT with fused embeddings, query / key norms and clipping used together: against plain PyTorch on
+the CPU, tensor parallel against dense, and on the GPU against the CPU model."""
+import copy
+
+import pytest
+import torch
+import torch.nn.functional as F
+from test_tensor_parallel import _run
+
+from determined_clone_amd.models import gpt2
+from determined_clone_amd.models.gpt2_tp import TPGPT
+from determined_clone_amd.ops import _grad
+from determined_clone_amd.ops import optim as fopt
+from determined_clone_amd.ops import transformer as T
+from determined_clone_amd.parallel import tensor as tp
+
+
+def _plain(model: gpt2.GPT, idx: torch.Tensor) -> torch.Tensor:
+    """The network in plain PyTorch; query and key heads normed when the model norms them."""
+    cfg = model.cfg
+    B, S = idx.shape
+    x = F.embedding(idx, model.wte.weight)
+    if model.wpe is not None:
+        x = x + model.wpe.weight[:S]
+    for blk in model.blocks:
+        h = F.layer_norm(x, (cfg.d_model,), blk.ln1.weight, blk.ln1.bias, cfg.ln_eps)
+        q, k, v = F.linear(h, blk.attn.qkv.weight, blk.attn.qkv.bias).view(B, S, 3, cfg.n_head, cfg.head_dim).unbind(2)
+        if cfg.qk_norm:
+            q = F.rms_norm(q, (cfg.head_dim,), blk.attn.q_norm.weight, cfg.ln_eps)
+            k = F.rms_norm(k, (cfg.head_dim,), blk.attn.k_norm.weight, cfg.ln_eps)
+        if blk.attn.rot:
+            q, k = (T.reference_rope(t, model.rope_cos, model.rope_sin, blk.attn.rot) for t in (q, k))
+        o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True)
+        x = x + F.linear(o.transpose(1, 2).reshape(B, S, -1), blk.attn.proj.weight, blk.attn.proj.bias)
+        h = F.layer_norm(x, (cfg.d_model,), blk.ln2.weight, blk.ln2.bias, cfg.ln_eps)
+        h = F.gelu(F.linear(h, blk.mlp.fc.weight, blk.mlp.fc.bias), approximate="tanh")
+        x = x + F.linear(h, blk.mlp.proj.weight, blk.mlp.proj.bias)
+    x = F.layer_norm(x, (cfg.d_model,), model.ln_f.weight, model.ln_f.bias, cfg.ln_eps)
+    return F.linear(x, model.wte.weight)
+
+
+def _model(pos, qk_norm=True, **kw):
+    torch.manual_seed(0)
+    m = gpt2.gpt2("tiny", pos_emb=pos, qk_norm=qk_norm, max_seq_len=160, **kw)
+    with torch.no_grad():
+        for n, p in m.named_parameters():
+            if "_norm.weight" in n:
+                p.uniform_(0.5, 1.5)
+    return m
+
+
+@pytest.mark.parametrize("pos", ["learned", "rotary"])
+def test_qk_norm_model_and_gradients_match_plain(pos):
+    m = _model(pos)
+    assert {k for k in m.state_dict() if "_norm" in k} == {f"blocks.{i}.attn.{n}_norm.weight" for i in (0, 1) for n in "qk"}
+    idx, tgt = torch.randint(0, 512, (2, 33)), torch.randint(0, 512, (2, 33))
+    logits, loss = m(idx, tgt)
+    want = _plain(m, idx)
+    torch.testing.assert_close(logits, want, atol=1e-4, rtol=1e-4)
+    got = torch.autograd.grad(loss, list(m.parameters()))
+    ref = torch.autograd.grad(F.cross_entropy(want.flatten(0, 1), tgt.flatten()), list(m.parameters()))
+    for (n, _), a, b in zip(m.named_parameters(), got, ref):
+        torch.testing.assert_close(a, b, atol=1e-6, rtol=1e-3, msg=n)
+
+
+def test_without_qk_norm_nothing_is_added():
+    assert not any("_norm" in k for k in gpt2.gpt2("tiny").state_dict())
+    m = gpt2.cast_for_mi355x(_model("rotary"))
+    assert m.blocks[0].attn.q_norm.weight.dtype == torch.float32  # kept like LayerNorm's
+
+
+def _tp_parity(rank, world, d, pos):
+    torch.manual_seed(0)
+    cfg = gpt2.config_for("tiny", n_layer=2, n_head=4, d_model=256, vocab_size=500, max_seq_len=32, pos_emb=pos,
+                          qk_norm=True)
+    full = gpt2.GPT(cfg)
+    with torch.no_grad():
+        for n, p in full.named_parameters():
+            if "_norm.weight" in n:
+                p.uniform_(0.5, 1.5)
+    grid = tp.ModelParallelGrid(model_parallel_size=world)
+    m = TPGPT(cfg, grid.get_model_parallel_group()).load_from(full)
+    g = torch.Generator().manual_seed(1)
+    idx = torch.randint(0, cfg.vocab_size, (2, 32), generator=g)
+    tgt = torch.randint(0, cfg.vocab_size, (2, 32), generator=g)
+    _, ref = full(idx, tgt)
+    ref.backward()
+    _, loss = m(idx, tgt)
+    loss.backward()
+    torch.testing.assert_close(loss, ref, rtol=1e-5, atol=1e-5)
+    for b, fb in zip(m.blocks, full.blocks):
+        for n in ("q_norm", "k_norm"):
+            torch.testing.assert_close(getattr(b.attn, n).weight.grad, getattr(fb.attn, n).weight.grad,
+                                       rtol=1e-4, atol=1e-7)
+    s, n = m.wte.start, m.wte.per
+    torch.testing.assert_close(m.wte.weight.grad, full.wte.weight.grad[s:s + n], rtol=1e-4, atol=1e-6)
+    sd = m.full_state_dict()
+    for k, v in full.state_dict().items():
+        torch.testing.assert_close(sd[k], v, msg=k)
+
+
+@pytest.mark.parametrize("pos", ["learned", "rotary"])
+def test_tensor_parallel_matches_dense(pos):
+    _run(2, _tp_parity, pos)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pos,qk_norm", [("learned", True), ("rotary", True), ("learned", False), ("rotary", False)])
+def test_a_training_step_on_the_gpu(pos, qk_norm):
+    """Lookup, norms, attention, loss, all gradients and clipping in bf16 against fp32 plain PyTorch
+    (bf16 activations through two blocks: 5 % of a gradient's norm)."""
+    m = _model(pos, qk_norm).cuda()
+    idx, tgt = (torch.randint(0, 512, (3, 150), device="cuda") for _ in range(2))
+    mb = gpt2.cast_for_mi355x(copy.deepcopy(m))
+    m.load_state_dict({k: v.float() for k, v in mb.state_dict().items()}, strict=False)
+    loss = F.cross_entropy(_plain(m, idx).flatten(0, 1), tgt.flatten())
+    loss.backward()
+    _, lb = mb(idx, tgt)
+    lb.backward()
+    assert abs(lb.item() - loss.item()) < 2e-2
+    for (n, p), q in zip(m.named_parameters(), mb.parameters()):
+        assert ((q.grad.float() - p.grad).norm() / p.grad.norm()).item() < 5e-2, n
+    want = torch.nn.utils.clip_grad_norm_(m.parameters(), 0.1)
+    got = fopt.clip_grad_norm_(mb.parameters(), 0.1)
+    assert abs(float(got) / float(want) - 1) < 2e-2
+    # bf16 gradients are rounded to 2^-8 after scaling, which averages out in the norm
+    assert abs(float(fopt.grad_norm(p.grad for p in mb.parameters())) - 0.1) < 1e-4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pos", ["learned", "rotary"])
+def test_gradients_added_in_place_are_the_returned_ones(pos):
+    """With the fused optimizer's flat gradients the kernels add into ``.grad``: two backward passes
+    give the sum of two plain ones, up to the rounding of the bf16 sums (two steps of 2^-8)."""
+    m = gpt2.cast_for_mi355x(_model(pos)).cuda()
+    flat = copy.deepcopy(m)
+    opt = fopt.FusedAdamW(flat.parameters(), lr=1e-3)
+    opt.space.ensure_views()
+    opt.zero_grad()
+    sums = None
+    for seed in (1, 2):
+        torch.manual_seed(seed)
+        idx, tgt = (torch.randint(0, 512, (2, 100), device="cuda") for _ in range(2))
+        got = torch.autograd.grad(m(idx, tgt)[1], list(m.parameters()))
+        sums = [g.double() for g in got] if sums is None else [s + g.double() for s, g in zip(sums, got)]
+        flat(idx, tgt)[1].backward()
+    _grad.join()
+    for (n, p), s in zip(flat.named_parameters(), sums):
+        assert ((p.grad.double() - s).norm() / s.norm()).item() < 2 * 2 ** -8, n
+
+
+@pytest.mark.gpu
+def test_training_with_a_torch_optimizer_and_the_kernels_clipping():
+    """Steps of a torch optimizer with clipping between: parameters follow torch's own clipping."""
+    a = gpt2.cast_for_mi355x(_model("rotary")).cuda()
+    b = copy.deepcopy(a)
+    oa, ob = (torch.optim.SGD(m.parameters(), lr=0.1) for m in (a, b))
+    for k in range(3):
+        torch.manual_seed(k)
+        idx = torch.randint(0, 512, (2, 64), device="cuda")
+        for m, o, clip in ((a, oa, fopt.clip_grad_norm_), (b, ob, torch.nn.utils.clip_grad_norm_)):
+            o.zero_grad()
+            m(idx, idx)[1].backward()
+            clip(m.parameters(), 0.5)
+            o.step()
+    for (n, p), q in zip(a.named_parameters(), b.named_parameters()):
+        # torch rounds the coefficient to bf16, which moves an update by up to 2^-8 and a bf16
+        # parameter by a step; fp32 parameters (norms, around 1) by updates of at most 0.05 * 2^-8
+        torch.testing.assert_close(p, q[1], rtol=2 ** -7, atol=3e-4, msg=n)
