@@ -37,15 +37,14 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-// What a lane keeps for its NV vectors of V features: their columns, the partner columns, the
-// weights and, for the current token, the angles (sin with the sign of the partner's term).
+// The columns of a lane's NV vectors of V features.
 template <int V, int NV>
 struct Lane {
   int col[NV];    // -1: past D
-  int other[NV];  // partner column, -1: not rotated
+  int other[NV];  // the rotation's partner column, -1: not rotated
 };
 
-template <typename T, int V, int L, int NV>
+template <int V, int L, int NV>
 __device__ __forceinline__ Lane<V, NV> lane_columns(int D, int rot) {
   Lane<V, NV> a;
   const int l = threadIdx.x & (L - 1), half = rot / 2;
@@ -64,18 +63,27 @@ __device__ __forceinline__ void load_f32(const float* p, int64_t at, float (&out
   for (int k = 0; k < V; ++k) out[k] = p[at + k];
 }
 
-// Angles of token t: row `at` of the tables, NaN when it has no row there.
+// Angles of a token: y = x cs + x[partner] sn, with sn's sign for this half of the pair (`sign` -1
+// turns back). Features that do not turn have cs 1, sn 0; a position without a table row gives NaN.
 template <int V, int NV>
 __device__ __forceinline__ void load_angles(const QkShape& s, const float* __restrict__ cosT,
                                             const float* __restrict__ sinT, int64_t b, int64_t tok,
                                             const Lane<V, NV>& a, float sign, float (&cs)[NV][V],
                                             float (&sn)[NV][V]) {
-  if (s.rot == 0) return;
-  const int64_t at = s.pos.p ? s.pos.at(b * s.pos_sb + tok) : tok;
-  const bool ok = static_cast<uint64_t>(at) < static_cast<uint64_t>(s.table_rows);
+  int64_t at = 0;
+  bool ok = true;
+  if (s.rot) {
+    at = s.pos.p ? s.pos.at(b * s.pos_sb + tok) : tok;
+    ok = static_cast<uint64_t>(at) < static_cast<uint64_t>(s.table_rows);
+  }
   const int half = s.rot / 2;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      cs[i][k] = 1.f;
+      sn[i][k] = 0.f;
+    }
     if (a.other[i] < 0) continue;
     const bool low = a.other[i] > a.col[i];
     const int64_t c = at * half + (low ? a.col[i] : a.other[i]);
@@ -83,27 +91,35 @@ __device__ __forceinline__ void load_angles(const QkShape& s, const float* __res
       load_f32<V>(cosT, c, cs[i]);
       load_f32<V>(sinT, c, sn[i]);
     }
+    const float f = ok ? (low ? -sign : sign) : __builtin_nanf("");
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      cs[i][k] = ok ? cs[i][k] : __builtin_nanf("");
-      sn[i][k] = ok ? (low ? -sign : sign) * sn[i][k] : __builtin_nanf("");
+      sn[i][k] *= f;
+      if (!ok) cs[i][k] = f;
     }
   }
+}
+
+// 1 / sqrt(mean + eps): v_rsq_f32 is within 1 ulp, below the rounding of the sum that it takes.
+__device__ __forceinline__ float rms_inv(float sum, float inv_d, float eps) {
+  return __builtin_amdgcn_rsqf(sum * inv_d + eps);
 }
 
 __device__ __forceinline__ int64_t head_offset(const HeadView& v, int64_t b, int64_t t, int h) {
   return b * v.sb + t * v.ss + h * v.sh;
 }
 
-template <typename T, int V, int L, int NV>
+// U groups of heads at once: their loads leave together, before the first is used.
+template <typename T, int V, int L, int NV, int U>
 __global__ __launch_bounds__(kQkBlock) void qk_fwd_kernel(QkShape s, HeadView xq, HeadView xk, HeadView yq,
                                                           HeadView yk, const float* __restrict__ wq,
                                                           const float* __restrict__ wk,
                                                           const float* __restrict__ cosT,
                                                           const float* __restrict__ sinT) {
   constexpr int G = 64 / L;  // heads at a time
-  const Lane<V, NV> a = lane_columns<T, V, L, NV>(s.D, s.rot);
+  const Lane<V, NV> a = lane_columns<V, L, NV>(s.D, s.rot);
   const int group = (threadIdx.x & 63) / L;
+  const float inv_d = 1.f / static_cast<float>(s.D);
   const int64_t tokens = s.B * s.S, step = static_cast<int64_t>(gridDim.x) * kQkWaves;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * kQkWaves + (threadIdx.x >> 6); t < tokens; t += step) {
     const int64_t b = t / s.S, tok = t - b * s.S;
@@ -114,47 +130,68 @@ __global__ __launch_bounds__(kQkBlock) void qk_fwd_kernel(QkShape s, HeadView xq
       const HeadView& x = which ? xk : xq;
       const HeadView& y = which ? yk : yq;
       const float* __restrict__ w = which ? wk : wq;
-      for (int h = group + static_cast<int>(blockIdx.y) * G; h < s.heads[which]; h += G * static_cast<int>(gridDim.y)) {
-        const int64_t xo = head_offset(x, b, tok, h), yo = head_offset(y, b, tok, h);
-        RawVec<T, V> rx[NV], ro[NV];
-        float ss = 0.f;
+      const int heads = s.heads[which];
+      // the weights go into the angles: y = r (x (w cs) + x[partner] (w[partner] sn))
+      float cw[NV][V], sw[NV][V];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          if (a.col[i] >= 0) rx[i] = ldv<T, V>(x.p, xo + a.col[i]);
-          if (a.other[i] >= 0) ro[i] = ldv<T, V>(x.p, xo + a.other[i]);
+      for (int i = 0; i < NV; ++i) {
+        float wv[V], wo[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) wv[k] = wo[k] = 1.f;
+        if (w && a.col[i] >= 0) load_f32<V>(w, a.col[i], wv);
+        if (w && a.other[i] >= 0) load_f32<V>(w, a.other[i], wo);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          cw[i][k] = wv[k] * cs[i][k];
+          sw[i][k] = wo[k] * sn[i][k];
         }
+      }
+      const int64_t x0 = b * x.sb + tok * x.ss, y0 = b * y.sb + tok * y.ss;
+      for (int h0 = group + static_cast<int>(blockIdx.y) * G * U; h0 < heads; h0 += G * U * static_cast<int>(gridDim.y)) {
+        RawVec<T, V> rx[U][NV], ro[U][NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          if (a.col[i] < 0) continue;
-          float v[V];
-          unpackv<T, V>(rx[i], v);
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * G;
+          const int64_t xo = x0 + h * x.sh;
 #pragma unroll
-          for (int k = 0; k < V; ++k) ss += v[k] * v[k];
-        }
-        const float r = 1.f / sqrtf(group_sum<L>(ss) / static_cast<float>(s.D) + s.eps);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          if (a.col[i] < 0) continue;
-          float v[V], wv[V];
-          unpackv<T, V>(rx[i], v);
-          if (w) load_f32<V>(w, a.col[i], wv);
-#pragma unroll
-          for (int k = 0; k < V; ++k) v[k] *= w ? r * wv[k] : r;
-          if (a.other[i] >= 0) {
-            float o[V];
-            unpackv<T, V>(ro[i], o);
-            if (w) load_f32<V>(w, a.other[i], wv);
-#pragma unroll
-            for (int k = 0; k < V; ++k) v[k] = v[k] * cs[i][k] + o[k] * (w ? r * wv[k] : r) * sn[i][k];
+          for (int i = 0; i < NV; ++i) {
+            rx[u][i] = ro[u][i] = RawVec<T, V>{};
+            if (h < heads && a.col[i] >= 0) rx[u][i] = ldv<T, V>(x.p, xo + a.col[i]);
+            if (h < heads && a.other[i] >= 0) ro[u][i] = ldv<T, V>(x.p, xo + a.other[i]);
           }
-          stv<T, V>(y.p, yo + a.col[i], packv<T, V>(v));
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * G;
+          if (h >= heads) break;
+          float v[NV][V], ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            float o[V];
+            unpackv<T, V>(rx[u][i], v[i]);
+            unpackv<T, V>(ro[u][i], o);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+              ss += v[i][k] * v[i][k];
+              v[i][k] = v[i][k] * cw[i][k] + o[k] * sw[i][k];
+            }
+          }
+          const float r = rms_inv(group_sum<L>(ss), inv_d, s.eps);
+          const int64_t yo = y0 + h * y.sh;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            if (a.col[i] < 0) continue;
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[i][k] *= r;
+            stv<T, V>(y.p, yo + a.col[i], packv<T, V>(v[i]));
+          }
         }
       }
     }
   }
 }
 
-template <typename T, int V, int L, int NV>
+template <typename T, int V, int L, int NV, int U>
 __global__ __launch_bounds__(kQkBlock) void qk_bwd_kernel(QkShape s, HeadView gq, HeadView gk, HeadView xq,
                                                           HeadView xk, HeadView dq, HeadView dk,
                                                           const float* __restrict__ wq,
@@ -164,16 +201,23 @@ __global__ __launch_bounds__(kQkBlock) void qk_bwd_kernel(QkShape s, HeadView gq
                                                           float* __restrict__ partial) {
   constexpr int G = 64 / L;
   __shared__ float red[kQkWaves][L * NV * V];
-  const Lane<V, NV> a = lane_columns<T, V, L, NV>(s.D, s.rot);
+  const Lane<V, NV> a = lane_columns<V, L, NV>(s.D, s.rot);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane / L;
+  const float inv_d = 1.f / static_cast<float>(s.D);
   const int64_t tokens = s.B * s.S, step = static_cast<int64_t>(gridDim.x) * kQkWaves;
-  float dw[2][NV][V];
+  float dw[2][NV][V], wv[2][NV][V];
 #pragma unroll
   for (int which = 0; which < 2; ++which)
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) dw[which][i][k] = 0.f;
+      for (int k = 0; k < V; ++k) {
+        dw[which][i][k] = 0.f;
+        wv[which][i][k] = 1.f;
+      }
+      const float* __restrict__ w = which ? wk : wq;
+      if (w && a.col[i] >= 0) load_f32<V>(w, a.col[i], wv[which][i]);
+    }
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * kQkWaves + wave; t < tokens; t += step) {
     const int64_t b = t / s.S, tok = t - b * s.S;
     float cs[NV][V], sn[NV][V];
@@ -183,54 +227,55 @@ __global__ __launch_bounds__(kQkBlock) void qk_bwd_kernel(QkShape s, HeadView gq
       const HeadView& x = which ? xk : xq;
       const HeadView& y = which ? gk : gq;
       const HeadView& d = which ? dk : dq;
-      const float* __restrict__ w = which ? wk : wq;
-      for (int h = group + static_cast<int>(blockIdx.y) * G; h < s.heads[which]; h += G * static_cast<int>(gridDim.y)) {
-        const int64_t xo = head_offset(x, b, tok, h), yo = head_offset(y, b, tok, h);
-        RawVec<T, V> rx[NV], rg[NV], ro[NV];
+      const int heads = s.heads[which];
+      const int64_t x0 = b * x.sb + tok * x.ss, y0 = b * y.sb + tok * y.ss, d0 = b * d.sb + tok * d.ss;
+      for (int h0 = group + static_cast<int>(blockIdx.y) * G * U; h0 < heads; h0 += G * U * static_cast<int>(gridDim.y)) {
+        RawVec<T, V> rx[U][NV], rg[U][NV], ro[U][NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          if (a.col[i] >= 0) {
-            rx[i] = ldv<T, V>(x.p, xo + a.col[i]);
-            rg[i] = ldv<T, V>(y.p, yo + a.col[i]);
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * G;
+          const int64_t xo = x0 + h * x.sh, yo = y0 + h * y.sh;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            rx[u][i] = rg[u][i] = ro[u][i] = RawVec<T, V>{};
+            if (h < heads && a.col[i] >= 0) {
+              rg[u][i] = ldv<T, V>(y.p, yo + a.col[i]);
+              rx[u][i] = ldv<T, V>(x.p, xo + a.col[i]);
+            }
+            if (h < heads && a.other[i] >= 0) ro[u][i] = ldv<T, V>(y.p, yo + a.other[i]);
           }
-          if (a.other[i] >= 0) ro[i] = ldv<T, V>(y.p, yo + a.other[i]);
         }
-        float g[NV][V], ss = 0.f, dot = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          if (a.col[i] < 0) continue;
-          float v[V];
-          unpackv<T, V>(rx[i], v);
-          unpackv<T, V>(rg[i], g[i]);
-          if (a.other[i] >= 0) {
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * G;
+          if (h >= heads) break;
+          float g[NV][V], v[NV][V], ss = 0.f, dot = 0.f;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
             float o[V];
-            unpackv<T, V>(ro[i], o);
+            unpackv<T, V>(rx[u][i], v[i]);
+            unpackv<T, V>(rg[u][i], g[i]);
+            unpackv<T, V>(ro[u][i], o);
 #pragma unroll
-            for (int k = 0; k < V; ++k) g[i][k] = g[i][k] * cs[i][k] + o[k] * sn[i][k];
+            for (int k = 0; k < V; ++k) {
+              g[i][k] = g[i][k] * cs[i][k] + o[k] * sn[i][k];
+              ss += v[i][k] * v[i][k];
+              dot += g[i][k] * wv[which][i][k] * v[i][k];
+            }
           }
-          float wv[V];
-          if (w) load_f32<V>(w, a.col[i], wv);
+          const float r = rms_inv(group_sum<L>(ss), inv_d, s.eps);
+          const float m = group_sum<L>(dot) * inv_d * r * r;  // mean(g w n) r
+          const int64_t at = d0 + h * d.sh;
 #pragma unroll
-          for (int k = 0; k < V; ++k) {
-            ss += v[k] * v[k];
-            dot += (w ? g[i][k] * wv[k] : g[i][k]) * v[k];
+          for (int i = 0; i < NV; ++i) {
+            if (a.col[i] < 0) continue;
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+              dw[which][i][k] += g[i][k] * (v[i][k] * r);
+              v[i][k] = r * (g[i][k] * wv[which][i][k] - v[i][k] * m);
+            }
+            stv<T, V>(d.p, at + a.col[i], packv<T, V>(v[i]));
           }
-        }
-        const float r = 1.f / sqrtf(group_sum<L>(ss) / static_cast<float>(s.D) + s.eps);
-        const float m = group_sum<L>(dot) / static_cast<float>(s.D) * r * r;  // mean(g w n) r
-        const int64_t o = head_offset(d, b, tok, h);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          if (a.col[i] < 0) continue;
-          float v[V], wv[V];
-          unpackv<T, V>(rx[i], v);
-          if (w) load_f32<V>(w, a.col[i], wv);
-#pragma unroll
-          for (int k = 0; k < V; ++k) {
-            dw[which][i][k] += g[i][k] * (v[k] * r);
-            v[k] = r * ((w ? g[i][k] * wv[k] : g[i][k]) - v[k] * m);
-          }
-          stv<T, V>(d.p, o + a.col[i], packv<T, V>(v));
         }
       }
     }
@@ -256,20 +301,27 @@ __global__ __launch_bounds__(kQkBlock) void qk_bwd_kernel(QkShape s, HeadView gq
   }
 }
 
-// dw[c] (+)= sum of the partial rows of q (columns 0 .. D-1) or k (the rest), 16 waves, fixed order
-constexpr int kSumWaves = 16;
-__global__ __launch_bounds__(kSumWaves * 64) void qk_dw_kernel(const float* __restrict__ partial, int rows, int D,
-                                                               ColumnOut q, ColumnOut k) {
-  __shared__ float red[kSumWaves][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+// dw[c] (+)= sum of the partial rows of q (columns 0 .. D-1) or k (the rest): 16 columns a workgroup,
+// its 64 lane groups of 16 take every 64th row, in a fixed order.
+constexpr int kSumCols = 16;
+__global__ __launch_bounds__(1024) void qk_dw_kernel(const float* __restrict__ partial, int rows, int D,
+                                                     ColumnOut q, ColumnOut k) {
+  constexpr int kSlices = 1024 / kSumCols;
+  __shared__ float red[kSlices][kSumCols];
+  const int slice = threadIdx.x / kSumCols, col = threadIdx.x % kSumCols, c = blockIdx.x * kSumCols + col;
   float a = 0.f;
-  if (c < 2 * D)
-#pragma unroll 4
-    for (int i = w; i < rows; i += kSumWaves) a += partial[static_cast<int64_t>(i) * 2 * D + c];
-  red[w][lane] = a;
+  if (c < 2 * D) {
+#pragma unroll 8
+    for (int i = slice; i < rows; i += kSlices) a += partial[static_cast<int64_t>(i) * 2 * D + c];
+  }
+  red[slice][col] = a;
   __syncthreads();
-  if (w || c >= 2 * D) return;
-  for (int i = 1; i < kSumWaves; ++i) a += red[i][lane];
+  for (int n = kSlices / 2; n > 0; n >>= 1) {
+    if (slice < n) red[slice][col] += red[slice + n][col];
+    __syncthreads();
+  }
+  if (slice || c >= 2 * D) return;
+  a = red[0][col];
   const ColumnOut& o = c < D ? q : k;
   const int j = c < D ? c : c - D;
   if (!o.p0) return;
@@ -316,14 +368,17 @@ void dispatch_all(TDtype dt, int vec_bytes, int D, F&& f) {
   }
 }
 
-// Workgroups: a wave a token up to kMaxBlocks of them, and several workgroups a token (over its
-// heads) while tokens alone leave the chip empty. `backward` writes a partial row per workgroup.
-constexpr int kMaxBlocks = 2048;
-dim3 qk_grid(const QkShape& s, int heads_at_once) {
+// Groups of heads at once: rows that take one vector per lane have registers for several.
+constexpr int unroll_of(int L, int NV, int most) { return NV > 1 ? 1 : (L > 16 ? 2 : most); }
+
+// Workgroups: a wave a token up to `most` of them, and several workgroups a token (over its heads)
+// while tokens alone leave the chip empty. The backward writes a partial row per workgroup.
+constexpr int kFwdBlocks = 8192, kBwdBlocks = 1024;
+dim3 qk_grid(const QkShape& s, int heads_at_once, int most) {
   int64_t x = (s.B * s.S + kQkWaves - 1) / kQkWaves;
-  x = x < 1 ? 1 : (x > kMaxBlocks ? kMaxBlocks : x);
-  const int most = s.heads[0] > s.heads[1] ? s.heads[0] : s.heads[1];
-  int64_t y = (most + heads_at_once - 1) / heads_at_once;
+  x = x < 1 ? 1 : (x > most ? most : x);
+  const int heads = s.heads[0] > s.heads[1] ? s.heads[0] : s.heads[1];
+  int64_t y = (heads + heads_at_once - 1) / heads_at_once;
   if (y > 256 / x) y = 256 / x;
   if (y < 1) y = 1;
   return dim3(static_cast<unsigned>(x), static_cast<unsigned>(y));
@@ -334,15 +389,15 @@ void qk_norm_rope_fwd(TDtype dt, int vec_bytes, const QkShape& s, const HeadView
                       const float* const w[2], const float* cosT, const float* sinT, hipStream_t st) {
   if (s.B * s.S == 0 || s.heads[0] + s.heads[1] == 0 || s.D == 0) return;
   dispatch_all(dt, vec_bytes, s.D, [&](auto t, auto v, auto l, auto nv) {
-    constexpr int L = decltype(l)::value;
-    hipLaunchKernelGGL((qk_fwd_kernel<decltype(t), decltype(v)::value, L, decltype(nv)::value>),
-                       qk_grid(s, 64 / L), dim3(kQkBlock), 0, st, s, x[0], x[1], y[0], y[1], w[0], w[1], cosT,
+    constexpr int L = decltype(l)::value, NV = decltype(nv)::value, U = unroll_of(L, NV, 4);
+    hipLaunchKernelGGL((qk_fwd_kernel<decltype(t), decltype(v)::value, L, NV, U>),
+                       qk_grid(s, 64 / L * U, kFwdBlocks), dim3(kQkBlock), 0, st, s, x[0], x[1], y[0], y[1], w[0], w[1], cosT,
                        sinT);
   });
 }
 
 int64_t qk_norm_rope_partial_floats(const QkShape& s) {
-  const dim3 g = qk_grid(s, 1);  // at least as many workgroups as any variant launches
+  const dim3 g = qk_grid(s, 1, kBwdBlocks);  // at least as many workgroups as any variant launches
   return static_cast<int64_t>(g.x) * g.y * 2 * s.D;
 }
 
@@ -353,16 +408,16 @@ void qk_norm_rope_bwd(TDtype dt, int vec_bytes, const QkShape& s, const HeadView
   int rows = 0;
   if (s.B * s.S > 0 && s.heads[0] + s.heads[1] > 0 && s.D > 0) {
     dispatch_all(dt, vec_bytes, s.D, [&](auto t, auto v, auto l, auto nv) {
-      constexpr int L = decltype(l)::value;
-      const dim3 grid = qk_grid(s, 64 / L);
+      constexpr int L = decltype(l)::value, NV = decltype(nv)::value, U = unroll_of(L, NV, 2);
+      const dim3 grid = qk_grid(s, 64 / L * U, kBwdBlocks);
       rows = static_cast<int>(grid.x * grid.y);
-      hipLaunchKernelGGL((qk_bwd_kernel<decltype(t), decltype(v)::value, L, decltype(nv)::value>), grid,
+      hipLaunchKernelGGL((qk_bwd_kernel<decltype(t), decltype(v)::value, L, NV, U>), grid,
                          dim3(kQkBlock), 0, st, s, dy[0], dy[1], x[0], x[1], dx[0], dx[1], w[0], w[1], cosT,
                          sinT, want ? partial : nullptr);
     });
   }
   if (!want || s.D == 0) return;
-  hipLaunchKernelGGL(qk_dw_kernel, dim3((2 * s.D + 63) / 64), dim3(kSumWaves * 64), 0, st, partial, rows, s.D,
+  hipLaunchKernelGGL(qk_dw_kernel, dim3((2 * s.D + kSumCols - 1) / kSumCols), dim3(1024), 0, st, partial, rows, s.D,
                      dw[0] ? *dw[0] : ColumnOut{}, dw[1] ? *dw[1] : ColumnOut{});
 }
 }  // namespace dca
