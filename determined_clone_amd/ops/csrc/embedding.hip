@@ -2,15 +2,18 @@
 //
 // Forward: out[t] = scale * W[id_t] + P[pos_t] in fp32, rounded once.
 //
-// Gradient: dW[v] = scale * sum_{t: id_t = v} dy[t]. The ids are sorted (stably, so that a token's
-// rows are added in token order and the result does not depend on scheduling), and workgroups take
-// equal ranges of the SORTED order: a frequent token is spread over as many workgroups as its rows
-// need, a rare one costs one row. A token inside one range is written once; one that crosses ranges
-// leaves fp32 partial rows which a second kernel joins in order. No float atomics.
+// Gradient: dW[v] = scale * sum_{t: id_t = v} dy[t], without float atomics, so that the result does
+// not depend on scheduling. Up to kDirectIds ids: a wave per table row looks through all ids and adds
+// the rows of those that are its own, in order. More ids are sorted by row (stably), and workgroups
+// take equal ranges of the SORTED order: a frequent token is spread over as many workgroups as its
+// rows need, a rare one costs one row. A token inside one range is written once; one that crosses
+// ranges leaves fp32 partial rows which a second kernel joins in order.
 //
-// The sort is a least-significant-digit radix sort of chunks in LDS (one workgroup a chunk), and
-// merges of up to 16 sorted chunks in which every element finds its rank by binary searches: ids
-// are few (16k-64k) beside the rows they index, so what counts is launches and latency.
+// The sort is one launch: workgroup b owns the rows whose low bits are b (256 workgroups, so that
+// frequent tokens, which have low ids in most vocabularies, fall to different ones), reads ALL ids,
+// counts those of lower workgroups (its place in the result) and its own by row and wave, and writes
+// its own out in order. Reading the ids once per workgroup (256 kB from L2 at 32k ids) costs less than
+// the passes and the launches of a sort that moves them.
 #include "embedding_api.h"
 
 namespace dca {
@@ -67,191 +70,218 @@ __global__ __launch_bounds__(kFwdBlock) void embed_fwd_kernel(
 }
 
 // ------------------------------------------------------------------ sort
-// An entry is row << 32 | token index: all entries differ, and their order is the stable one.
-constexpr int kSortItems = 4;
-constexpr int kSortChunk = 1024 * kSortItems;
-constexpr int kDigits = 256;
-constexpr int kMergeWays = 16;
-
+// An entry is row << 32 | token index. Ids without a row (another shard's, mistakes) are left out.
 __device__ __forceinline__ int row_of(uint64_t entry) { return static_cast<int>(entry >> 32); }
 
-// Sorts one chunk of ids per workgroup by row, least significant digit first. Per digit every wave
-// counts its own items in order (lanes with equal digits find each other by ballots), one scan over
-// (digit, wave) turns counts into places, and the items move through LDS. Rows past the table
-// (other shards, mistakes, the padding of the last chunk) take the key `rows`, after all others.
-__global__ __launch_bounds__(1024) void embed_sort_kernel(EmbedIds ids, uint64_t* __restrict__ out, int bits) {
-  __shared__ uint64_t buf[kSortChunk];
-  __shared__ uint32_t count[16 * kDigits];
-  __shared__ uint32_t wave_total[16];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * kSortChunk;
-  const int n = static_cast<int>(ids.n - base < kSortChunk ? ids.n - base : kSortChunk);
-  const uint64_t below = (1ull << lane) - 1;
-  volatile uint32_t* mine = count + w * kDigits;  // volatile: a wave's own reads and writes stay in order
-  uint32_t key[kSortItems], at[kSortItems];
-#pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
-    const int l = (w * kSortItems + j) * 64 + lane;
-    key[j] = static_cast<uint32_t>(ids.rows);
-    at[j] = static_cast<uint32_t>(base + l);
-    if (l < n) {
-      const int64_t id = ids.ids.at(base + l) - ids.start;
-      if (static_cast<uint64_t>(id) < static_cast<uint64_t>(ids.rows)) key[j] = static_cast<uint32_t>(id);
-    }
-  }
-  for (int shift = 0; shift < bits; shift += 8) {
-#pragma unroll
-    for (int i = 0; i < kDigits / 64; ++i) mine[i * 64 + lane] = 0;
-    uint32_t rank[kSortItems];
-#pragma unroll
-    for (int j = 0; j < kSortItems; ++j) {
-      const uint32_t d = (key[j] >> shift) & (kDigits - 1);
-      uint64_t same = ~0ull;
-#pragma unroll
-      for (int b = 0; b < 8; ++b) {
-        const bool one = (d >> b) & 1;
-        const uint64_t v = __ballot(one);
-        same &= one ? v : ~v;
-      }
-      const uint32_t before = static_cast<uint32_t>(__popcll(same & below));
-      const uint32_t had = mine[d];
-      rank[j] = had + before;
-      if (before == 0) mine[d] = had + static_cast<uint32_t>(__popcll(same));
-    }
-    __syncthreads();
-    // exclusive scan over (digit, wave): thread t takes digit t / 4, waves 4 (t % 4) .. + 3
-    const int sd = tid >> 2, sw = (tid & 3) * 4;
-    uint32_t c[4], sum = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      c[i] = count[(sw + i) * kDigits + sd];
-      sum += c[i];
-    }
-    uint32_t incl = sum;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint32_t v = __shfl_up(incl, off, 64);
-      if (lane >= off) incl += v;
-    }
-    if (lane == 63) wave_total[w] = incl;
-    __syncthreads();
-    uint32_t place = incl - sum;
-    for (int i = 0; i < w; ++i) place += wave_total[i];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      count[(sw + i) * kDigits + sd] = place;
-      place += c[i];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kSortItems; ++j)
-      buf[count[w * kDigits + ((key[j] >> shift) & (kDigits - 1))] + rank[j]] =
-          static_cast<uint64_t>(key[j]) << 32 | at[j];
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kSortItems; ++j) {
-      const uint64_t e = buf[(w * kSortItems + j) * 64 + lane];
-      key[j] = static_cast<uint32_t>(e >> 32);
-      at[j] = static_cast<uint32_t>(e);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
-    const int l = (w * kSortItems + j) * 64 + lane;
-    if (l < n) out[base + l] = static_cast<uint64_t>(key[j]) << 32 | at[j];
-  }
+constexpr int kPlaceUnroll = 8;
+constexpr int kFlagWords = 16;
+
+// 16 bytes of zeros at a time, the last bytes one by one; `p` is 16-byte aligned.
+__device__ __forceinline__ void zero_fill(void* p, int64_t bytes, int64_t first, int64_t step) {
+  const int64_t n = bytes / 16;
+  for (int64_t i = first; i < n; i += step) static_cast<uint4*>(p)[i] = make_uint4(0, 0, 0, 0);
+  if (first < bytes % 16) static_cast<char*>(p)[n * 16 + first] = 0;
 }
 
-// Merges groups of up to kMergeWays sorted runs of `len`: an element's place is its own index plus
-// the number of smaller elements in each of the group's other runs.
-__global__ __launch_bounds__(256) void embed_merge_kernel(const uint64_t* __restrict__ in,
-                                                          uint64_t* __restrict__ out, int64_t n,
-                                                          int64_t len) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= n) return;
-  const uint64_t v = in[i];
-  const int64_t run = i / len;
-  const int64_t g0 = run / kMergeWays * kMergeWays;  // the group's first run
-  int64_t place = g0 * len + (i - run * len);
-  int64_t top = 1;
-  while (top * 2 <= len) top *= 2;
-#pragma unroll 4
-  for (int k = 0; k < kMergeWays; ++k) {
-    const int64_t r0 = (g0 + k) * len;
-    const int64_t m = n - r0 < len ? n - r0 : len;
-    if (m <= 0 || g0 + k == run) continue;
-    int64_t below = 0;
-    for (int64_t step = top; step > 0; step >>= 1)
-      if (below + step <= m && in[r0 + below + step - 1] < v) below += step;
-    place += below;
+// Workgroups [0, owners): the sort; b owns rows r with r mod 2^shift = b, kRows of them at most. The
+// others clear `clear` meanwhile. A wave walks through its stretch of the ids twice, 64 at a time:
+// first counting, then placing; the second walk skips the steps whose flag says that none of the 64
+// was this workgroup's (three of four). What bounds it is the instructions per id of the first walk.
+template <typename I, int kRows, int kWaves>
+__global__ __launch_bounds__(kWaves * 64) void embed_place_kernel(const I* __restrict__ ids, int64_t n, int64_t start,
+                                                                  int64_t rows, int shift,
+                                                                  uint64_t* __restrict__ sorted,
+                                                                  int64_t* __restrict__ total, int owners,
+                                                                  void* __restrict__ clear, int64_t clear_bytes) {
+  constexpr int kThreads = kWaves * 64, kEach = kRows * kWaves / kThreads;
+  if (static_cast<int>(blockIdx.x) >= owners) {
+    zero_fill(clear, clear_bytes, static_cast<int64_t>(blockIdx.x - owners) * kThreads + threadIdx.x,
+              static_cast<int64_t>(gridDim.x - owners) * kThreads);
+    return;
   }
-  out[place] = v;
+  __shared__ uint32_t count[kWaves * kRows];
+  __shared__ uint32_t wave_sum[2][kWaves];
+  __shared__ uint64_t flags[kWaves][kFlagWords];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t me = blockIdx.x, mask = (1u << shift) - 1;
+  // steps of 64 ids for a wave, a multiple of the unrolled loops' (what is past n counts nowhere)
+  const int64_t steps = (n + kThreads * kPlaceUnroll - 1) / (kThreads * kPlaceUnroll) * kPlaceUnroll;
+  const int64_t lo = w * steps * 64;
+  volatile uint32_t* mine = count + w * kRows;  // volatile: a wave's own reads and writes stay in order
+#pragma unroll
+  for (int i = 0; i < kRows / 64; ++i) mine[i * 64 + lane] = 0;
+  uint32_t below = 0;
+  for (int64_t s0 = 0; s0 < steps; s0 += 64) {
+    uint64_t flag = 0;
+    const int m = static_cast<int>(steps - s0 < 64 ? steps - s0 : 64);
+    for (int j = 0; j < m; j += kPlaceUnroll) {
+      const int64_t first = lo + (s0 + j) * 64;
+      if (first >= n) break;
+      I id[kPlaceUnroll];
+      if (first + 64 * kPlaceUnroll <= n) {
+#pragma unroll
+        for (int u = 0; u < kPlaceUnroll; ++u) id[u] = ids[first + u * 64 + lane];
+      } else {
+#pragma unroll
+        for (int u = 0; u < kPlaceUnroll; ++u)
+          id[u] = first + u * 64 + lane < n ? ids[first + u * 64 + lane] : static_cast<I>(start - 1);
+      }
+      uint32_t mine_in = 0;
+#pragma unroll
+      for (int u = 0; u < kPlaceUnroll; ++u) {
+        const int64_t row = static_cast<int64_t>(id[u]) - start;
+        const bool ok = static_cast<uint64_t>(row) < static_cast<uint64_t>(rows);
+        const uint32_t r = static_cast<uint32_t>(row), owner = r & mask;
+        below += ok && owner < me;
+        const bool own = ok && owner == me;
+        if (own) atomicAdd(&count[w * kRows + (r >> shift)], 1u);
+        mine_in |= __ballot(own) ? 1u << u : 0u;
+      }
+      flag |= static_cast<uint64_t>(mine_in) << j;
+    }
+    if (s0 / 64 < kFlagWords) flags[w][s0 / 64] = flag;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) below += __shfl_xor(below, off, 64);
+  if (lane == 0) wave_sum[0][w] = below;
+  __syncthreads();
+  // exclusive scan over (row, wave), from the number of lower workgroups' ids on
+  uint32_t c[kEach], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int e = tid * kEach + i;
+    c[i] = count[e % kWaves * kRows + e / kWaves];
+    sum += c[i];
+  }
+  uint32_t incl = sum;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t v = __shfl_up(incl, off, 64);
+    if (lane >= off) incl += v;
+  }
+  if (lane == 63) wave_sum[1][w] = incl;
+  __syncthreads();
+  uint32_t place = incl - sum;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) place += wave_sum[0][i] + (i < w ? wave_sum[1][i] : 0);
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int e = tid * kEach + i;
+    count[e % kWaves * kRows + e / kWaves] = place;
+    place += c[i];
+  }
+  if (static_cast<int>(blockIdx.x) == owners - 1 && tid == kThreads - 1) *total = place;
+  __syncthreads();
+  const uint64_t lower = (1ull << lane) - 1;
+  for (int64_t s0 = 0; s0 < steps; s0 += 64) {
+    const int64_t left = steps - s0;
+    uint64_t flag = left < 64 ? (1ull << left) - 1 : ~0ull;
+    if (s0 / 64 < kFlagWords) flag = flags[w][s0 / 64];
+    const uint32_t flag_lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(flag));
+    const uint32_t flag_hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(flag >> 32));
+    flag = static_cast<uint64_t>(flag_hi) << 32 | flag_lo;
+    while (flag) {
+      I id[kPlaceUnroll];
+      int64_t first[kPlaceUnroll];
+#pragma unroll
+      for (int u = 0; u < kPlaceUnroll; ++u) {  // the flags run out: n, whose ids are nobody's
+        first[u] = flag ? lo + (s0 + __builtin_ctzll(flag)) * 64 : n;
+        flag &= flag - 1;
+        const int64_t i = first[u] + lane;
+        id[u] = ids[i < n ? i : n - 1];
+      }
+#pragma unroll
+      for (int u = 0; u < kPlaceUnroll; ++u) {
+        const int64_t row = static_cast<int64_t>(id[u]) - start;
+        const uint32_t r = static_cast<uint32_t>(row);
+        const bool own = first[u] + lane < n && static_cast<uint64_t>(row) < static_cast<uint64_t>(rows) &&
+                         (r & mask) == me;
+        uint64_t left_own = __ballot(own), same = 0;
+        // lanes with the same row: a row at a time, and bit by bit where a step has many rows
+        for (int k = 0; k < 3 && left_own; ++k) {
+          const uint64_t s = __ballot(own && r == static_cast<uint32_t>(__builtin_amdgcn_readlane(r, __builtin_ctzll(left_own))));
+          if (s >> lane & 1) same = s;
+          left_own &= ~s;
+        }
+        if (left_own) {
+          const bool rest = left_own >> lane & 1;
+          uint64_t s = left_own;
+          for (int b = 0; (kRows >> b) > 1; ++b) {
+            const bool one = (r >> shift >> b) & 1;
+            const uint64_t v = __ballot(one);
+            s &= one ? v : ~v;
+          }
+          if (rest) same = s;
+        }
+        if (own) {
+          const uint32_t before = static_cast<uint32_t>(__popcll(same & lower)), to = mine[r >> shift];
+          if (before == 0) mine[r >> shift] = to + static_cast<uint32_t>(__popcll(same));
+          sorted[to + before] = static_cast<uint64_t>(r) << 32 | static_cast<uint32_t>(first[u] + lane);
+        }
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------------ gradient
-constexpr int kGradUnroll = 8;
-
 __device__ __forceinline__ int64_t partial_stride(int E) { return (E + 3) & ~3; }
 
+// out = scale a, or scale a + old
 template <typename T, int V>
-__device__ __forceinline__ void grad_store(void* out, int64_t at, float (&a)[V], float scale, bool accumulate) {
+__device__ __forceinline__ void grad_store(void* out, int64_t at, float (&a)[V], float scale, bool accumulate,
+                                           const RawVec<T, V>& old) {
+  float o[V];
+  unpackv<T, V>(old, o);
 #pragma unroll
-  for (int k = 0; k < V; ++k) a[k] *= scale;
-  if (accumulate) {
-    float old[V];
-    unpackv<T, V>(ldv<T, V>(out, at), old);
-#pragma unroll
-    for (int k = 0; k < V; ++k) a[k] += old[k];
+  for (int k = 0; k < V; ++k) {
+    a[k] *= scale;
+    if (accumulate) a[k] += o[k];
   }
   stv<T, V>(out, at, packv<T, V>(a));
 }
-
-// Workgroup x takes sorted entries [x K, (x + 1) K), workgroup y a stretch of columns. partial
-// holds two rows a workgroup: 0 the sum of a token that began in an earlier range (its "head"),
-// 1 of one that began here and goes on (its "tail").
 template <typename T, int V>
-__global__ __launch_bounds__(256) void embed_grad_kernel(const uint64_t* __restrict__ sorted,
-                                                         const void* __restrict__ dy, void* __restrict__ out,
-                                                         float* __restrict__ partial, int64_t n, int64_t rows,
-                                                         int E, int K, float scale, bool accumulate) {
-  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
+__device__ __forceinline__ void grad_store(void* out, int64_t at, float (&a)[V], float scale, bool accumulate) {
+  RawVec<T, V> old{};
+  if (accumulate) old = ldv<T, V>(out, at);
+  grad_store<T, V>(out, at, a, scale, accumulate, old);
+}
+
+// Few ids: a wave per table row and stretch of 64 V columns. Rows without an id are cleared (or left
+// alone when adding), so that this is the gradient's only launch.
+constexpr int kDirectIds = 512;
+constexpr int kDirectWaves = 4;
+constexpr int kDirectUnroll = 8;
+template <typename T, int V>
+__global__ __launch_bounds__(kDirectWaves * 64) void embed_grad_direct_kernel(
+    EmbedIds ids, const void* __restrict__ dy, void* __restrict__ out, int E, float scale, bool accumulate) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kDirectWaves + (threadIdx.x >> 6);
+  if (row >= ids.rows) return;
+  const int c = (blockIdx.y * 64 + lane) * V;
   const bool ok = c < E;
-  const int64_t lo = static_cast<int64_t>(blockIdx.x) * K;
-  const int64_t hi = lo + K < n ? lo + K : n;
-  const int64_t ps = partial_stride(E);
-  float* head = partial + static_cast<int64_t>(blockIdx.x) * 2 * ps;
-  int row = row_of(sorted[lo]);
-  bool open = lo > 0 && row_of(sorted[lo - 1]) == row;
+  const int n = static_cast<int>(ids.n);
   float a[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) a[k] = 0.f;
-  auto put = [&](float* to) {
-    if (!ok) return;
+  bool any = false;
+#pragma unroll 2
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    uint64_t own = __ballot(i0 + lane < n && ids.ids.at(i0 + lane) - ids.start == row);
+    any |= own != 0;
+    while (own) {
+      RawVec<T, V> r[kDirectUnroll];
+      int got = 0;
 #pragma unroll
-    for (int k = 0; k < V; ++k) to[c + k] = a[k];
-  };
-  for (int64_t e = lo; e < hi; e += kGradUnroll) {
-    if (row_of(sorted[e]) >= rows) break;  // rows of no table: all that follow are, too
-    uint64_t s[kGradUnroll];
-    RawVec<T, V> r[kGradUnroll];
-#pragma unroll
-    for (int u = 0; u < kGradUnroll; ++u) s[u] = sorted[e + u < hi ? e + u : hi - 1];
-#pragma unroll
-    for (int u = 0; u < kGradUnroll; ++u)
-      if (ok) r[u] = ldv<T, V>(dy, static_cast<int64_t>(s[u] & 0xffffffffu) * E + c);
-#pragma unroll
-    for (int u = 0; u < kGradUnroll; ++u) {
-      if (e + u >= hi) continue;
-      const int next = row_of(s[u]);
-      if (next != row) {
-        if (open) put(head);
-        else if (ok && row < rows) grad_store<T, V>(out, static_cast<int64_t>(row) * E + c, a, scale, accumulate);
-#pragma unroll
-        for (int k = 0; k < V; ++k) a[k] = 0.f;
-        row = next;
-        open = false;
+      for (int u = 0; u < kDirectUnroll; ++u) {
+        if (!own) break;
+        const int t = i0 + __builtin_ctzll(own);
+        own &= own - 1;
+        if (ok) r[u] = ldv<T, V>(dy, static_cast<int64_t>(t) * E + c);
+        ++got;
       }
-      if (ok) {
+#pragma unroll
+      for (int u = 0; u < kDirectUnroll; ++u) {
+        if (u >= got || !ok) break;
         float x[V];
         unpackv<T, V>(r[u], x);
 #pragma unroll
@@ -259,10 +289,86 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const uint64_t* __restr
       }
     }
   }
-  if (row >= rows) return;
-  if (open) put(head);
-  else if (hi < n && row_of(sorted[hi]) == row) put(head + ps);
-  else if (ok) grad_store<T, V>(out, static_cast<int64_t>(row) * E + c, a, scale, accumulate);
+  if (ok && (any || !accumulate)) grad_store<T, V>(out, row * E + c, a, scale, accumulate);
+}
+
+// Workgroup x takes sorted entries [x K, (x + 1) K), K <= 64, workgroup y a stretch of columns. Every
+// wave holds the range's entries in its lanes, so all row addresses are known from the start; the
+// next rows' loads (and, when adding, of the table rows that end among them) leave before the present
+// ones are added. partial holds two rows a workgroup: 0 the
+// sum of a token that began in an earlier range (its "head"), 1 of one that began here and goes on
+// (its "tail").
+constexpr int kGradUnroll = 8;
+template <typename T, int V, bool kAdd>
+__global__ __launch_bounds__(256) void embed_grad_kernel(const uint64_t* __restrict__ sorted,
+                                                         const int64_t* __restrict__ total,
+                                                         const void* __restrict__ dy, void* out,
+                                                         float* __restrict__ partial, int E, int K, float scale) {
+  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
+  const bool ok = c < E;
+  const int64_t lo = static_cast<int64_t>(blockIdx.x) * K, n = *total;
+  if (lo >= n) return;
+  const int cnt = static_cast<int>(n - lo < K ? n - lo : K);
+  const int64_t ps = partial_stride(E);
+  float* head = partial + static_cast<int64_t>(blockIdx.x) * 2 * ps;
+  const int lane = threadIdx.x & 63;
+  const uint64_t entry = sorted[lo + (lane < cnt ? lane : cnt - 1)];
+  const int before = lo > 0 ? row_of(sorted[lo - 1]) : -1;
+  const int after = lo + cnt < n ? row_of(sorted[lo + cnt]) : -1;
+  const int row_l = row_of(entry);
+  const uint32_t tok_l = static_cast<uint32_t>(entry);
+  auto row_at = [&](int e) { return e < cnt ? __builtin_amdgcn_readlane(row_l, e) : after; };
+  bool open = before == row_at(0);
+  float a[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) a[k] = 0.f;
+  struct Batch {
+    RawVec<T, V> dy[kGradUnroll], old[kAdd ? kGradUnroll : 1];
+  };
+  auto load = [&](Batch& r, int e) {
+#pragma unroll
+    for (int u = 0; u < kGradUnroll; ++u) {
+      if (e + u >= cnt) break;
+      const uint32_t tok = __builtin_amdgcn_readlane(tok_l, e + u);
+      if (ok) r.dy[u] = ldv<T, V>(dy, static_cast<int64_t>(tok) * E + c);
+      if constexpr (kAdd) {
+        const int row = row_at(e + u);
+        if (ok && row != row_at(e + u + 1)) r.old[u] = ldv<T, V>(out, static_cast<int64_t>(row) * E + c);
+      }
+    }
+  };
+  Batch now, then;
+  load(now, 0);
+  for (int e = 0; e < cnt; e += kGradUnroll) {
+    if (e + kGradUnroll < cnt) load(then, e + kGradUnroll);
+#pragma unroll
+    for (int u = 0; u < kGradUnroll; ++u) {
+      if (e + u >= cnt) break;
+      if (ok) {
+        float x[V];
+        unpackv<T, V>(now.dy[u], x);
+#pragma unroll
+        for (int k = 0; k < V; ++k) a[k] += x[k];
+      }
+      const int row = row_at(e + u);
+      const bool last = e + u + 1 == cnt, ends = row != row_at(e + u + 1);
+      if (!ends && !last) continue;
+      // the token ends here, or goes on in the next range
+      if (ok) {
+        if (open || !ends) {
+          float* to = open ? head : head + ps;
+#pragma unroll
+          for (int k = 0; k < V; ++k) to[c + k] = a[k];
+        } else {
+          grad_store<T, V>(out, static_cast<int64_t>(row) * E + c, a, scale, kAdd, now.old[kAdd ? u : 0]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) a[k] = 0.f;
+      open = false;
+    }
+    now = then;
+  }
 }
 
 // Joins the tokens that cross ranges: the workgroup in whose range a token begins adds the heads of
@@ -270,16 +376,16 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const uint64_t* __restr
 constexpr int kJoinWaves = 4;
 template <typename T>
 __global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(const uint64_t* __restrict__ sorted,
+                                                                     const int64_t* __restrict__ total,
                                                                      const float* __restrict__ partial,
-                                                                     void* __restrict__ out, int64_t n,
-                                                                     int64_t rows, int E, int K, float scale,
-                                                                     bool accumulate) {
+                                                                     void* __restrict__ out, int E, int K,
+                                                                     float scale, bool accumulate) {
   __shared__ float4 red[kJoinWaves][64];
-  const int64_t lo = static_cast<int64_t>(blockIdx.x) * K, hi = lo + K;
+  const int64_t lo = static_cast<int64_t>(blockIdx.x) * K, hi = lo + K, n = *total;
   if (hi >= n) return;
   const int row = row_of(sorted[hi - 1]);
-  if (row >= rows || row_of(sorted[hi]) != row) return;                                  // ends here
-  if (lo > 0 && row_of(sorted[lo]) == row && row_of(sorted[lo - 1]) == row) return;      // began earlier
+  if (row_of(sorted[hi]) != row) return;                                             // ends here
+  if (lo > 0 && row_of(sorted[lo]) == row && row_of(sorted[lo - 1]) == row) return;  // began earlier
   // the last range that holds the token: doubling steps, then halving ones
   const int64_t x = blockIdx.x, nb = (n + K - 1) / K;
   int64_t last = x + 1, step = 1;  // range `last` begins with the token
@@ -294,7 +400,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(const uint6
   const int64_t ps = partial_stride(E);
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   if (c < E) {
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t b = x + 1 + w; b <= last; b += kJoinWaves) {
       const float4 p = *reinterpret_cast<const float4*>(partial + b * 2 * ps + c);
       a.x += p.x; a.y += p.y; a.z += p.z; a.w += p.w;
@@ -393,26 +499,53 @@ void embed_fwd(TDtype dt, int vec_bytes, const EmbedIds& ids, const void* table,
   });
 }
 
-int64_t embed_grad_workspace(int64_t n, int E) { return 2 * n * 8 + partial_floats(n, E) * 4 + 16; }
+// The workspace: the number of sorted entries (16 bytes for it), the entries, the partial rows.
+int64_t embed_grad_workspace(int64_t n, int E) {
+  return n <= kDirectIds ? 0 : 16 + (n + 1) / 2 * 16 + partial_floats(n, E) * 4;
+}
+
+template <typename I, int kRows, int kWaves>
+static void place(const EmbedIds& ids, int shift, uint64_t* sorted, int64_t* total, void* clear,
+                  int64_t clear_bytes, hipStream_t st) {
+  const int owners = static_cast<int>(ids.rows < (1 << shift) ? ids.rows : 1 << shift);
+  int64_t clearing = (clear_bytes / 16 + kWaves * 64 - 1) / (kWaves * 64);
+  if (clearing > 2048) clearing = 2048;
+  if (clear_bytes && clearing < 1) clearing = 1;
+  hipLaunchKernelGGL((embed_place_kernel<I, kRows, kWaves>), dim3(static_cast<unsigned>(owners + clearing)),
+                     dim3(kWaves * 64), 0, st, static_cast<const I*>(ids.ids.p), ids.n, ids.start, ids.rows, shift,
+                     sorted, total, owners, clear, clear_bytes);
+}
+template <typename I>
+static void place(const EmbedIds& ids, uint64_t* sorted, int64_t* total, void* clear, int64_t clear_bytes,
+                  hipStream_t st) {
+  // a workgroup per CU, with counters for 256 or 1024 rows; more workgroups past 256k rows
+  int shift = 8;
+  while ((ids.rows - 1) >> shift >= 1024) ++shift;
+  if ((ids.rows - 1) >> shift < 256) place<I, 256, 16>(ids, shift, sorted, total, clear, clear_bytes, st);
+  else place<I, 1024, 8>(ids, shift, sorted, total, clear, clear_bytes, st);
+}
 
 void embed_grad(TDtype dt, int vec_bytes, const EmbedIds& ids, const void* dy, void* out, int E,
                 float scale, bool accumulate, void* workspace, hipStream_t st) {
   const int64_t n = ids.n;
-  if (n == 0 || E == 0) return;
-  uint64_t* a = static_cast<uint64_t*>(workspace);
-  uint64_t* b = a + n;
-  float* partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + (2 * n * 8 + 15) / 16 * 16);
-  int bits = 1;  // of the largest key, `rows` itself
-  while (bits < 32 && (ids.rows >> bits)) ++bits;
-  hipLaunchKernelGGL(embed_sort_kernel, dim3(static_cast<unsigned>((n + kSortChunk - 1) / kSortChunk)),
-                     dim3(1024), 0, st, ids, a, bits);
-  for (int64_t len = kSortChunk; len < n; len *= kMergeWays) {
-    hipLaunchKernelGGL(embed_merge_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, st,
-                       a, b, n, len);
-    uint64_t* t = a;
-    a = b;
-    b = t;
+  if (E == 0 || ids.rows == 0) return;
+  if (n <= kDirectIds) {
+    dispatch_tv(dt, vec_bytes, [&](auto t, auto v) {
+      using T = decltype(t);
+      constexpr int V = decltype(v)::value;
+      hipLaunchKernelGGL((embed_grad_direct_kernel<T, V>),
+                         dim3(static_cast<unsigned>((ids.rows + kDirectWaves - 1) / kDirectWaves),
+                              static_cast<unsigned>((E + 64 * V - 1) / (64 * V))),
+                         dim3(kDirectWaves * 64), 0, st, ids, dy, out, E, scale, accumulate);
+    });
+    return;
   }
+  int64_t* total = static_cast<int64_t*>(workspace);
+  uint64_t* sorted = static_cast<uint64_t*>(workspace) + 2;
+  float* partial = reinterpret_cast<float*>(sorted + (n + 1) / 2 * 2);
+  const int64_t clear = accumulate ? 0 : ids.rows * E * (dt == TDtype::kF32 ? 4 : 2);
+  if (ids.ids.is32) place<int32_t>(ids, sorted, total, out, clear, st);
+  else place<int64_t>(ids, sorted, total, out, clear, st);
   const int K = grad_range(n);
   const unsigned nb = static_cast<unsigned>((n + K - 1) / K);
   dispatch_tv(dt, vec_bytes, [&](auto t, auto v) {
@@ -420,11 +553,16 @@ void embed_grad(TDtype dt, int vec_bytes, const EmbedIds& ids, const void* dy, v
     constexpr int V = decltype(v)::value;
     const int nv = E / V;
     const int threads = nv >= 256 ? 256 : (nv + 63) / 64 * 64;
-    hipLaunchKernelGGL((embed_grad_kernel<T, V>), dim3(nb, static_cast<unsigned>((nv + threads - 1) / threads)),
-                       dim3(threads), 0, st, a, dy, out, partial, n, ids.rows, E, K, scale, accumulate);
+    const dim3 grid(nb, static_cast<unsigned>((nv + threads - 1) / threads));
+    if (accumulate)
+      hipLaunchKernelGGL((embed_grad_kernel<T, V, true>), grid, dim3(threads), 0, st, sorted, total, dy, out,
+                         partial, E, K, scale);
+    else
+      hipLaunchKernelGGL((embed_grad_kernel<T, V, false>), grid, dim3(threads), 0, st, sorted, total, dy, out,
+                         partial, E, K, scale);
     if (nb > 1)
       hipLaunchKernelGGL(embed_join_kernel<T>, dim3(nb, static_cast<unsigned>((E + 255) / 256)),
-                         dim3(kJoinWaves * 64), 0, st, a, partial, out, n, ids.rows, E, K, scale, accumulate);
+                         dim3(kJoinWaves * 64), 0, st, sorted, total, partial, out, E, K, scale, accumulate);
   });
 }
 

@@ -28,8 +28,9 @@ void embed_fwd(TDtype dt, int vec_bytes, const EmbedIds& ids, const void* table,
                const EmbedPos& pos, float scale, void* out, int E, hipStream_t st);
 // bytes of workspace embed_grad needs for n ids and rows of E
 int64_t embed_grad_workspace(int64_t n, int E);
-// out[row] (+)= scale * sum of dy's rows with that id; rows without an id are left as they are.
-// dy [n][E], out [rows][E], both contiguous.
+// out[row] = scale * sum of dy's rows with that id, zero for rows without one; `accumulate`: added to
+// what is there, rows without an id untouched. dy [n][E], out [rows][E] (16-byte aligned unless
+// accumulating), both contiguous.
 void embed_grad(TDtype dt, int vec_bytes, const EmbedIds& ids, const void* dy, void* out, int E,
                 float scale, bool accumulate, void* workspace, hipStream_t st);
 // out[j] (+)= sum_b dy[b][j] for dy [B][N]

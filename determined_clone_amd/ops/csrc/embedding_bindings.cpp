@@ -80,9 +80,9 @@ Tensor embed_fwd(const Tensor& idx, const Tensor& weight, const OptT& pos_weight
   return out;
 }
 
-// The gradient's destination: `acc` (added to) or a new zeroed table.
+// The gradient's destination: `acc` (added to) or a new table.
 Tensor destination(const OptT& acc, int64_t rows, int64_t E, const Tensor& dy) {
-  if (!given(acc)) return torch::zeros({rows, E}, dy.options());
+  if (!given(acc)) return torch::empty({rows, E}, dy.options());
   TORCH_CHECK(acc->is_contiguous() && acc->dim() == 2 && acc->size(0) == rows && acc->size(1) == E &&
                   acc->scalar_type() == dy.scalar_type() && acc->device() == dy.device(),
               "embedding: the accumulation target must be contiguous and like the table");
@@ -99,7 +99,7 @@ Tensor embed_grad(const Tensor& dy_in, const Tensor& idx, int64_t rows, double s
   const int64_t E = dy.size(-1);
   const dca::EmbedIds ids = ids_of(idx, dy, rows, start, true);
   Tensor out = destination(acc, rows, E, dy);
-  if (idx.numel() == 0 || E == 0) return out;
+  if (E == 0) return out;
   Tensor ws = torch::empty({dca::embed_grad_workspace(ids.n, static_cast<int>(E))}, dy.options().dtype(at::kByte));
   dca::WidestVec vec(static_cast<int>(dy.element_size()));
   vec.elems(E);
@@ -118,13 +118,8 @@ Tensor embed_pos_grad(const Tensor& dy_in, int64_t rows, const OptT& acc) {
   Tensor dy = dy_in.contiguous();
   const int64_t S = dy.size(-2), E = dy.size(-1), N = S * E;
   const int64_t filled = dy.numel() ? S : 0;
-  Tensor out;
-  if (given(acc)) {
-    out = destination(acc, rows, E, dy);
-  } else {
-    out = torch::empty({rows, E}, dy.options());
-    if (filled < rows) out.narrow(0, filled, rows - filled).zero_();
-  }
+  Tensor out = destination(acc, rows, E, dy);
+  if (!given(acc) && filled < rows) out.narrow(0, filled, rows - filled).zero_();
   if (dy.numel() == 0) return out;
   dca::WidestVec vec(static_cast<int>(dy.element_size()));
   vec.elems(N);
