@@ -22,11 +22,13 @@ namespace {
 // ------------------------------------------------------------------ forward
 constexpr int kFwdBlock = 256;
 constexpr int kFwdUnroll = 4;
+// Outputs past the L2s are streamed (67 MB: 20.2 against 22.1 us), smaller ones stay for their reader.
+constexpr int64_t kStreamBytes = 32 << 20;
 
 template <typename T, int V>
 __global__ __launch_bounds__(kFwdBlock) void embed_fwd_kernel(
     EmbedIds ids, const void* __restrict__ table, int64_t stride, EmbedPos pos, float scale,
-    void* __restrict__ out, int E, int rows_per_block) {
+    void* __restrict__ out, int E, int rows_per_block, bool stream) {
   const unsigned nv = static_cast<unsigned>(E / V);
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * rows_per_block;
   const int64_t left = ids.n - t0;
@@ -64,82 +66,94 @@ __global__ __launch_bounds__(kFwdBlock) void embed_fwd_kernel(
 #pragma unroll
         for (int k = 0; k < V; ++k) a[k] = pok[u] ? a[k] + b[k] : __builtin_nanf("");
       }
-      stv<T, V>(out, t0 * E + static_cast<int64_t>(i) * V, packv<T, V>(a));
+      const int64_t to = t0 * E + static_cast<int64_t>(i) * V;
+      if (stream) stv_nt<T, V>(out, to, packv<T, V>(a));
+      else stv<T, V>(out, to, packv<T, V>(a));
     }
   }
 }
 
 // ------------------------------------------------------------------ sort
-// An entry is row << 32 | token index. Ids without a row (another shard's, mistakes) are left out.
+// An entry is row << 32 | token index; ids without a row (another shard's, mistakes) have row -1.
 __device__ __forceinline__ int row_of(uint64_t entry) { return static_cast<int>(entry >> 32); }
 
 constexpr int kPlaceUnroll = 8;
-constexpr int kFlagWords = 16;
+constexpr int kList = 256;
 
-// 16 bytes of zeros at a time, the last bytes one by one; `p` is 16-byte aligned.
+// 16 bytes of zeros at a time, the last bytes one by one; `p` is 16-byte aligned. Streamed, and dy read
+// that way by the kernels that follow: 31x2047 tokens, E = 1600, fp16: 180 against 217 us altogether,
+// since their lines do not push each other's out of the caches half-written.
 __device__ __forceinline__ void zero_fill(void* p, int64_t bytes, int64_t first, int64_t step) {
   const int64_t n = bytes / 16;
-  for (int64_t i = first; i < n; i += step) static_cast<uint4*>(p)[i] = make_uint4(0, 0, 0, 0);
+  for (int64_t i = first; i < n; i += step) stnt16(static_cast<uint4*>(p) + i, make_uint4(0, 0, 0, 0));
   if (first < bytes % 16) static_cast<char*>(p)[n * 16 + first] = 0;
 }
 
-// Workgroups [0, owners): the sort; b owns rows r with r mod 2^shift = b, kRows of them at most. The
-// others clear `clear` meanwhile. A wave walks through its stretch of the ids twice, 64 at a time:
-// first counting, then placing; the second walk skips the steps whose flag says that none of the 64
-// was this workgroup's (three of four). What bounds it is the instructions per id of the first walk.
+// Workgroups [0, 2^shift): the sort; b owns the ids with b in their low bits, rows r with r mod 2^shift
+// = b and, behind them, the ids that have no row (counter kRows - 1). The others clear `clear`
+// meanwhile. A wave walks through its stretch of the ids, 64 at a time, counts, and lists its own in
+// LDS; after the scan it places those (with more than kList of them, by walking through its stretch
+// again). What bounds it is the instructions per id of the walk, which therefore looks at low bits
+// only: whether an id has a row is asked of the few that are the workgroup's own. 32k ids: 4.5 us for
+// the walk, beside 4 us of launch, scan and ends.
 template <typename I, int kRows, int kWaves>
 __global__ __launch_bounds__(kWaves * 64) void embed_place_kernel(const I* __restrict__ ids, int64_t n, int64_t start,
                                                                   int64_t rows, int shift,
                                                                   uint64_t* __restrict__ sorted,
-                                                                  int64_t* __restrict__ total, int owners,
                                                                   void* __restrict__ clear, int64_t clear_bytes) {
   constexpr int kThreads = kWaves * 64, kEach = kRows * kWaves / kThreads;
-  if (static_cast<int>(blockIdx.x) >= owners) {
+  const uint32_t owners = 1u << shift;
+  if (blockIdx.x >= owners) {
     zero_fill(clear, clear_bytes, static_cast<int64_t>(blockIdx.x - owners) * kThreads + threadIdx.x,
               static_cast<int64_t>(gridDim.x - owners) * kThreads);
     return;
   }
   __shared__ uint32_t count[kWaves * kRows];
   __shared__ uint32_t wave_sum[2][kWaves];
-  __shared__ uint64_t flags[kWaves][kFlagWords];
+  __shared__ uint32_t list[kWaves][kList];  // counter << 22 | index in the wave's stretch
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t me = blockIdx.x, mask = (1u << shift) - 1;
+  const uint32_t me = blockIdx.x, mask = owners - 1, start_lo = static_cast<uint32_t>(start);
+  auto counter_of = [&](I id) {
+    const int64_t row = static_cast<int64_t>(id) - start;
+    return static_cast<uint64_t>(row) < static_cast<uint64_t>(rows) ? static_cast<uint32_t>(row) >> shift : kRows - 1u;
+  };
   // steps of 64 ids for a wave, a multiple of the unrolled loops' (what is past n counts nowhere)
   const int64_t steps = (n + kThreads * kPlaceUnroll - 1) / (kThreads * kPlaceUnroll) * kPlaceUnroll;
   const int64_t lo = w * steps * 64;
   volatile uint32_t* mine = count + w * kRows;  // volatile: a wave's own reads and writes stay in order
 #pragma unroll
   for (int i = 0; i < kRows / 64; ++i) mine[i * 64 + lane] = 0;
+  const uint64_t lower = (1ull << lane) - 1;
   uint32_t below = 0;
-  for (int64_t s0 = 0; s0 < steps; s0 += 64) {
-    uint64_t flag = 0;
-    const int m = static_cast<int>(steps - s0 < 64 ? steps - s0 : 64);
-    for (int j = 0; j < m; j += kPlaceUnroll) {
-      const int64_t first = lo + (s0 + j) * 64;
-      if (first >= n) break;
-      I id[kPlaceUnroll];
-      if (first + 64 * kPlaceUnroll <= n) {
+  int64_t listed = 0;
+  for (int64_t j = 0; j < steps; j += kPlaceUnroll) {
+    const int64_t first = lo + j * 64;
+    if (first >= n) break;
+    I id[kPlaceUnroll];
+    const bool full = first + 64 * kPlaceUnroll <= n;
+    if (full) {
 #pragma unroll
-        for (int u = 0; u < kPlaceUnroll; ++u) id[u] = ids[first + u * 64 + lane];
-      } else {
+      for (int u = 0; u < kPlaceUnroll; ++u) id[u] = ids[first + u * 64 + lane];
+    } else {
 #pragma unroll
-        for (int u = 0; u < kPlaceUnroll; ++u)
-          id[u] = first + u * 64 + lane < n ? ids[first + u * 64 + lane] : static_cast<I>(start - 1);
-      }
-      uint32_t mine_in = 0;
-#pragma unroll
-      for (int u = 0; u < kPlaceUnroll; ++u) {
-        const int64_t row = static_cast<int64_t>(id[u]) - start;
-        const bool ok = static_cast<uint64_t>(row) < static_cast<uint64_t>(rows);
-        const uint32_t r = static_cast<uint32_t>(row), owner = r & mask;
-        below += ok && owner < me;
-        const bool own = ok && owner == me;
-        if (own) atomicAdd(&count[w * kRows + (r >> shift)], 1u);
-        mine_in |= __ballot(own) ? 1u << u : 0u;
-      }
-      flag |= static_cast<uint64_t>(mine_in) << j;
+      for (int u = 0; u < kPlaceUnroll; ++u) id[u] = first + u * 64 + lane < n ? ids[first + u * 64 + lane] : 0;
     }
-    if (s0 / 64 < kFlagWords) flags[w][s0 / 64] = flag;
+#pragma unroll
+    for (int u = 0; u < kPlaceUnroll; ++u) {
+      uint32_t owner = (static_cast<uint32_t>(id[u]) - start_lo) & mask;
+      if (!full && first + u * 64 + lane >= n) owner = ~0u;  // nobody's
+      below += owner < me;
+      const bool own = owner == me;
+      const uint64_t all = __builtin_amdgcn_ballot_w64(own);
+      if (!all) continue;
+      if (own) {
+        const uint32_t d = counter_of(id[u]);
+        atomicAdd(&count[w * kRows + d], 1u);
+        const int64_t at = listed + __popcll(all & lower);
+        if (at < kList) list[w][at] = d << 22 | static_cast<uint32_t>((j + u) * 64 + lane);
+      }
+      listed += __popcll(all);
+    }
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) below += __shfl_xor(below, off, 64);
@@ -170,55 +184,53 @@ __global__ __launch_bounds__(kWaves * 64) void embed_place_kernel(const I* __res
     count[e % kWaves * kRows + e / kWaves] = place;
     place += c[i];
   }
-  if (static_cast<int>(blockIdx.x) == owners - 1 && tid == kThreads - 1) *total = place;
   __syncthreads();
-  const uint64_t lower = (1ull << lane) - 1;
-  for (int64_t s0 = 0; s0 < steps; s0 += 64) {
-    const int64_t left = steps - s0;
-    uint64_t flag = left < 64 ? (1ull << left) - 1 : ~0ull;
-    if (s0 / 64 < kFlagWords) flag = flags[w][s0 / 64];
-    const uint32_t flag_lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(flag));
-    const uint32_t flag_hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(flag >> 32));
-    flag = static_cast<uint64_t>(flag_hi) << 32 | flag_lo;
-    while (flag) {
-      I id[kPlaceUnroll];
-      int64_t first[kPlaceUnroll];
-#pragma unroll
-      for (int u = 0; u < kPlaceUnroll; ++u) {  // the flags run out: n, whose ids are nobody's
-        first[u] = flag ? lo + (s0 + __builtin_ctzll(flag)) * 64 : n;
-        flag &= flag - 1;
-        const int64_t i = first[u] + lane;
-        id[u] = ids[i < n ? i : n - 1];
+  // places the lanes' own ids, `d` their counters, `at` their indexes
+  auto put = [&](bool own, uint32_t d, int64_t at) {
+    uint64_t left = __builtin_amdgcn_ballot_w64(own), same = 0;
+    // lanes with the same counter: one at a time, and bit by bit where there are many
+    for (int k = 0; k < 3 && left; ++k) {
+      const uint32_t one = __builtin_amdgcn_readlane(d, __builtin_ctzll(left));
+      const uint64_t s = __builtin_amdgcn_ballot_w64(own && d == one);
+      if (s >> lane & 1) same = s;
+      left &= ~s;
+    }
+    if (left) {
+      const bool rest = left >> lane & 1;
+      for (int b = 0; (kRows >> b) > 1; ++b) {
+        const bool one = (d >> b) & 1;
+        const uint64_t v = __builtin_amdgcn_ballot_w64(one);
+        left &= one ? v : ~v;
       }
+      if (rest) same = left;
+    }
+    if (own) {
+      const uint32_t before = static_cast<uint32_t>(__popcll(same & lower)), to = mine[d];
+      if (before == 0) mine[d] = to + static_cast<uint32_t>(__popcll(same));
+      const uint32_t row = d == kRows - 1u ? ~0u : d << shift | me;
+      sorted[to + before] = static_cast<uint64_t>(row) << 32 | static_cast<uint32_t>(at);
+    }
+  };
+  if (listed <= kList && steps * 64 <= 1 << 22) {
+    for (int64_t i = 0; i < listed; i += 64) {
+      const bool own = i + lane < listed;
+      const uint32_t e = own ? list[w][i + lane] : 0;
+      put(own, e >> 22, lo + (e & ((1u << 22) - 1)));
+    }
+    return;
+  }
+  for (int64_t j = 0; j < steps; j += kPlaceUnroll) {
+    if (lo + j * 64 >= n) break;
+    I id[kPlaceUnroll];
 #pragma unroll
-      for (int u = 0; u < kPlaceUnroll; ++u) {
-        const int64_t row = static_cast<int64_t>(id[u]) - start;
-        const uint32_t r = static_cast<uint32_t>(row);
-        const bool own = first[u] + lane < n && static_cast<uint64_t>(row) < static_cast<uint64_t>(rows) &&
-                         (r & mask) == me;
-        uint64_t left_own = __ballot(own), same = 0;
-        // lanes with the same row: a row at a time, and bit by bit where a step has many rows
-        for (int k = 0; k < 3 && left_own; ++k) {
-          const uint64_t s = __ballot(own && r == static_cast<uint32_t>(__builtin_amdgcn_readlane(r, __builtin_ctzll(left_own))));
-          if (s >> lane & 1) same = s;
-          left_own &= ~s;
-        }
-        if (left_own) {
-          const bool rest = left_own >> lane & 1;
-          uint64_t s = left_own;
-          for (int b = 0; (kRows >> b) > 1; ++b) {
-            const bool one = (r >> shift >> b) & 1;
-            const uint64_t v = __ballot(one);
-            s &= one ? v : ~v;
-          }
-          if (rest) same = s;
-        }
-        if (own) {
-          const uint32_t before = static_cast<uint32_t>(__popcll(same & lower)), to = mine[r >> shift];
-          if (before == 0) mine[r >> shift] = to + static_cast<uint32_t>(__popcll(same));
-          sorted[to + before] = static_cast<uint64_t>(r) << 32 | static_cast<uint32_t>(first[u] + lane);
-        }
-      }
+    for (int u = 0; u < kPlaceUnroll; ++u) {
+      const int64_t i = lo + (j + u) * 64 + lane;
+      id[u] = ids[i < n ? i : n - 1];
+    }
+#pragma unroll
+    for (int u = 0; u < kPlaceUnroll; ++u) {
+      const int64_t i = lo + (j + u) * 64 + lane;
+      put(i < n && ((static_cast<uint32_t>(id[u]) - start_lo) & mask) == me, counter_of(id[u]), i);
     }
   }
 }
@@ -301,13 +313,12 @@ __global__ __launch_bounds__(kDirectWaves * 64) void embed_grad_direct_kernel(
 constexpr int kGradUnroll = 8;
 template <typename T, int V, bool kAdd>
 __global__ __launch_bounds__(256) void embed_grad_kernel(const uint64_t* __restrict__ sorted,
-                                                         const int64_t* __restrict__ total,
                                                          const void* __restrict__ dy, void* out,
-                                                         float* __restrict__ partial, int E, int K, float scale) {
+                                                         float* __restrict__ partial, int64_t n, int E, int K,
+                                                         float scale) {
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
   const bool ok = c < E;
-  const int64_t lo = static_cast<int64_t>(blockIdx.x) * K, n = *total;
-  if (lo >= n) return;
+  const int64_t lo = static_cast<int64_t>(blockIdx.x) * K;
   const int cnt = static_cast<int>(n - lo < K ? n - lo : K);
   const int64_t ps = partial_stride(E);
   float* head = partial + static_cast<int64_t>(blockIdx.x) * 2 * ps;
@@ -330,10 +341,10 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const uint64_t* __restr
     for (int u = 0; u < kGradUnroll; ++u) {
       if (e + u >= cnt) break;
       const uint32_t tok = __builtin_amdgcn_readlane(tok_l, e + u);
-      if (ok) r.dy[u] = ldv<T, V>(dy, static_cast<int64_t>(tok) * E + c);
+      if (ok && row_at(e + u) >= 0) r.dy[u] = ldv_nt<T, V>(dy, static_cast<int64_t>(tok) * E + c);
       if constexpr (kAdd) {
         const int row = row_at(e + u);
-        if (ok && row != row_at(e + u + 1)) r.old[u] = ldv<T, V>(out, static_cast<int64_t>(row) * E + c);
+        if (ok && row >= 0 && row != row_at(e + u + 1)) r.old[u] = ldv<T, V>(out, static_cast<int64_t>(row) * E + c);
       }
     }
   };
@@ -344,13 +355,17 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const uint64_t* __restr
 #pragma unroll
     for (int u = 0; u < kGradUnroll; ++u) {
       if (e + u >= cnt) break;
+      const int row = row_at(e + u);
+      if (row < 0) {  // ids without a row
+        open = false;
+        continue;
+      }
       if (ok) {
         float x[V];
         unpackv<T, V>(now.dy[u], x);
 #pragma unroll
         for (int k = 0; k < V; ++k) a[k] += x[k];
       }
-      const int row = row_at(e + u);
       const bool last = e + u + 1 == cnt, ends = row != row_at(e + u + 1);
       if (!ends && !last) continue;
       // the token ends here, or goes on in the next range
@@ -376,26 +391,25 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const uint64_t* __restr
 constexpr int kJoinWaves = 4;
 template <typename T>
 __global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(const uint64_t* __restrict__ sorted,
-                                                                     const int64_t* __restrict__ total,
                                                                      const float* __restrict__ partial,
-                                                                     void* __restrict__ out, int E, int K,
-                                                                     float scale, bool accumulate) {
+                                                                     void* __restrict__ out, int64_t n, int E,
+                                                                     int K, float scale, bool accumulate) {
   __shared__ float4 red[kJoinWaves][64];
-  const int64_t lo = static_cast<int64_t>(blockIdx.x) * K, hi = lo + K, n = *total;
+  const int64_t lo = static_cast<int64_t>(blockIdx.x) * K, hi = lo + K;
   if (hi >= n) return;
-  const int row = row_of(sorted[hi - 1]);
-  if (row_of(sorted[hi]) != row) return;                                             // ends here
-  if (lo > 0 && row_of(sorted[lo]) == row && row_of(sorted[lo - 1]) == row) return;  // began earlier
-  // the last range that holds the token: doubling steps, then halving ones
+  const int row = row_of(sorted[hi - 1]), next = row_of(sorted[hi]), first = row_of(sorted[lo]);
+  const int before = row_of(sorted[lo > 0 ? lo - 1 : 0]);
+  if (row < 0 || next != row) return;                   // ends here
+  if (lo > 0 && first == row && before == row) return;  // began earlier
+  // the last range that begins with the token: 64 ranges a step, since a step costs a trip to memory
   const int64_t x = blockIdx.x, nb = (n + K - 1) / K;
-  int64_t last = x + 1, step = 1;  // range `last` begins with the token
-  while (last + step < nb && row_of(sorted[(last + step) * K]) == row) {
-    last += step;
-    step *= 2;
-  }
-  for (; step > 0; step >>= 1)
-    if (last + step < nb && row_of(sorted[(last + step) * K]) == row) last += step;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int64_t last = x;
+  for (uint64_t with = ~0ull; with == ~0ull;) {
+    const int64_t at = last + 1 + lane;
+    with = __builtin_amdgcn_ballot_w64(at < nb && row_of(sorted[at < nb ? at * K : 0]) == row);
+    last += __popcll(with);  // the ranges that begin with it follow each other
+  }
   const int c = (blockIdx.y * 64 + lane) * 4;
   const int64_t ps = partial_stride(E);
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -474,7 +488,8 @@ void dispatch_tv(TDtype dt, int vec_bytes, F&& f) {
   }
 }
 
-// Sorted entries a workgroup takes: enough workgroups to fill the chip, few partial rows.
+// Sorted entries a workgroup takes: enough workgroups to fill the chip, few partial rows (32k ids,
+// E = 1024, bf16, both kernels: 8 entries 42 us, 16 38 us, 32 33 us, 64 36 us).
 int grad_range(int64_t n) { return n >= 16384 ? 32 : (n >= 4096 ? 16 : 8); }
 
 int64_t partial_floats(int64_t n, int E) {
@@ -495,34 +510,33 @@ void embed_fwd(TDtype dt, int vec_bytes, const EmbedIds& ids, const void* table,
     if (r > ids.n / 1024) r = ids.n / 1024;
     if (r < 1) r = 1;
     hipLaunchKernelGGL((embed_fwd_kernel<T, V>), dim3(static_cast<unsigned>((ids.n + r - 1) / r)),
-                       dim3(kFwdBlock), 0, st, ids, table, stride, pos, scale, out, E, static_cast<int>(r));
+                       dim3(kFwdBlock), 0, st, ids, table, stride, pos, scale, out, E, static_cast<int>(r),
+                       ids.n * E * kElem<T> >= kStreamBytes);
   });
 }
 
-// The workspace: the number of sorted entries (16 bytes for it), the entries, the partial rows.
+// The workspace: the sorted entries, the partial rows.
 int64_t embed_grad_workspace(int64_t n, int E) {
-  return n <= kDirectIds ? 0 : 16 + (n + 1) / 2 * 16 + partial_floats(n, E) * 4;
+  return n <= kDirectIds ? 0 : (n + 1) / 2 * 16 + partial_floats(n, E) * 4;
 }
 
 template <typename I, int kRows, int kWaves>
-static void place(const EmbedIds& ids, int shift, uint64_t* sorted, int64_t* total, void* clear,
-                  int64_t clear_bytes, hipStream_t st) {
-  const int owners = static_cast<int>(ids.rows < (1 << shift) ? ids.rows : 1 << shift);
+static void place(const EmbedIds& ids, int shift, uint64_t* sorted, void* clear, int64_t clear_bytes,
+                  hipStream_t st) {
   int64_t clearing = (clear_bytes / 16 + kWaves * 64 - 1) / (kWaves * 64);
   if (clearing > 2048) clearing = 2048;
   if (clear_bytes && clearing < 1) clearing = 1;
-  hipLaunchKernelGGL((embed_place_kernel<I, kRows, kWaves>), dim3(static_cast<unsigned>(owners + clearing)),
+  hipLaunchKernelGGL((embed_place_kernel<I, kRows, kWaves>), dim3(static_cast<unsigned>((1 << shift) + clearing)),
                      dim3(kWaves * 64), 0, st, static_cast<const I*>(ids.ids.p), ids.n, ids.start, ids.rows, shift,
-                     sorted, total, owners, clear, clear_bytes);
+                     sorted, clear, clear_bytes);
 }
 template <typename I>
-static void place(const EmbedIds& ids, uint64_t* sorted, int64_t* total, void* clear, int64_t clear_bytes,
-                  hipStream_t st) {
-  // a workgroup per CU, with counters for 256 or 1024 rows; more workgroups past 256k rows
+static void place(const EmbedIds& ids, uint64_t* sorted, void* clear, int64_t clear_bytes, hipStream_t st) {
+  // a workgroup per CU, with counters for 255 or 1023 rows; more workgroups past 256k rows
   int shift = 8;
-  while ((ids.rows - 1) >> shift >= 1024) ++shift;
-  if ((ids.rows - 1) >> shift < 256) place<I, 256, 16>(ids, shift, sorted, total, clear, clear_bytes, st);
-  else place<I, 1024, 8>(ids, shift, sorted, total, clear, clear_bytes, st);
+  while ((ids.rows - 1) >> shift >= 1023) ++shift;
+  if ((ids.rows - 1) >> shift < 255) place<I, 256, 16>(ids, shift, sorted, clear, clear_bytes, st);
+  else place<I, 1024, 8>(ids, shift, sorted, clear, clear_bytes, st);
 }
 
 void embed_grad(TDtype dt, int vec_bytes, const EmbedIds& ids, const void* dy, void* out, int E,
@@ -540,12 +554,11 @@ void embed_grad(TDtype dt, int vec_bytes, const EmbedIds& ids, const void* dy, v
     });
     return;
   }
-  int64_t* total = static_cast<int64_t*>(workspace);
-  uint64_t* sorted = static_cast<uint64_t*>(workspace) + 2;
+  uint64_t* sorted = static_cast<uint64_t*>(workspace);
   float* partial = reinterpret_cast<float*>(sorted + (n + 1) / 2 * 2);
   const int64_t clear = accumulate ? 0 : ids.rows * E * (dt == TDtype::kF32 ? 4 : 2);
-  if (ids.ids.is32) place<int32_t>(ids, sorted, total, out, clear, st);
-  else place<int64_t>(ids, sorted, total, out, clear, st);
+  if (ids.ids.is32) place<int32_t>(ids, sorted, out, clear, st);
+  else place<int64_t>(ids, sorted, out, clear, st);
   const int K = grad_range(n);
   const unsigned nb = static_cast<unsigned>((n + K - 1) / K);
   dispatch_tv(dt, vec_bytes, [&](auto t, auto v) {
@@ -555,14 +568,14 @@ void embed_grad(TDtype dt, int vec_bytes, const EmbedIds& ids, const void* dy, v
     const int threads = nv >= 256 ? 256 : (nv + 63) / 64 * 64;
     const dim3 grid(nb, static_cast<unsigned>((nv + threads - 1) / threads));
     if (accumulate)
-      hipLaunchKernelGGL((embed_grad_kernel<T, V, true>), grid, dim3(threads), 0, st, sorted, total, dy, out,
-                         partial, E, K, scale);
+      hipLaunchKernelGGL((embed_grad_kernel<T, V, true>), grid, dim3(threads), 0, st, sorted, dy, out, partial,
+                         n, E, K, scale);
     else
-      hipLaunchKernelGGL((embed_grad_kernel<T, V, false>), grid, dim3(threads), 0, st, sorted, total, dy, out,
-                         partial, E, K, scale);
+      hipLaunchKernelGGL((embed_grad_kernel<T, V, false>), grid, dim3(threads), 0, st, sorted, dy, out, partial,
+                         n, E, K, scale);
     if (nb > 1)
       hipLaunchKernelGGL(embed_join_kernel<T>, dim3(nb, static_cast<unsigned>((E + 255) / 256)),
-                         dim3(kJoinWaves * 64), 0, st, sorted, total, partial, out, E, K, scale, accumulate);
+                         dim3(kJoinWaves * 64), 0, st, sorted, partial, out, n, E, K, scale, accumulate);
   });
 }
 

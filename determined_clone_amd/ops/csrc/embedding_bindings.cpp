@@ -5,6 +5,7 @@
 
 #include <limits>
 
+#include "autograd_util.h"
 #include "embedding_api.h"
 
 namespace {
@@ -128,10 +129,60 @@ Tensor embed_pos_grad(const Tensor& dy_in, int64_t rows, const OptT& acc) {
   dca::batch_sum(tdt(dy), vec.bytes(), dy.data_ptr(), out.data_ptr(), dy.numel() / N, N, given(acc), stream());
   return out;
 }
+
+// The operator with its gradient, as an autograd node here rather than in Python: a training step's
+// lookup is a few microseconds of GPU time, less than a Python node costs on the host.
+struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& idx_in, const Tensor& weight,
+                        const OptT& pos_weight, const OptT& positions_in, double scale, int64_t start, bool shard) {
+    const Tensor idx = idx_in.contiguous();
+    OptT positions, pos_rows;
+    if (given(positions_in)) positions = positions_in->expand(idx.sizes()).contiguous();
+    if (given(pos_weight)) pos_rows = rows_of(*pos_weight);
+    // the tables as they are now are not needed again (and may be updated or moved before the backward)
+    ctx->save_for_backward({idx, positions.has_value() ? *positions : Tensor()});
+    ctx->saved_data["weight"] = weight;
+    ctx->saved_data["pos_weight"] = given(pos_weight) ? *pos_weight : Tensor();
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["start"] = start;
+    return embed_fwd(idx, rows_of(weight), pos_rows, positions, scale, start, shard);
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &idx = saved[0], &positions = saved[1];
+    const Tensor weight = ctx->saved_data["weight"].toTensor(), pos_weight = ctx->saved_data["pos_weight"].toTensor();
+    const Tensor dy = grads[0].contiguous();
+    torch::autograd::variable_list out(7);
+    if (ctx->needs_input_grad(1)) {
+      const OptT acc = dca::grad_target(weight);
+      const Tensor dw = embed_grad(dy, idx, weight.size(0), ctx->saved_data["scale"].toDouble(),
+                                   ctx->saved_data["start"].toInt(), acc);
+      if (!given(acc)) out[1] = dw;
+    }
+    if (pos_weight.defined() && ctx->needs_input_grad(2)) {
+      const OptT acc = dca::grad_target(pos_weight);
+      const Tensor dp = positions.defined() ? embed_grad(dy, positions, pos_weight.size(0), 1.0, 0, acc)
+                                            : embed_pos_grad(dy, pos_weight.size(0), acc);
+      if (!given(acc)) out[2] = dp;
+    }
+    return dca::once(std::move(out), grads[0]);
+  }
+
+ private:
+  static Tensor rows_of(const Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous(); }
+};
+
+Tensor embedding(const Tensor& idx, const Tensor& weight, const OptT& pos_weight, const OptT& positions, double scale,
+                 int64_t start, bool shard) {
+  return EmbeddingNode::apply(idx, weight, pos_weight, positions, scale, start, shard);
+}
 }  // namespace
 
 void register_embedding_ops(pybind11::module& m) {
   namespace py = pybind11;
+  m.def("embedding", &embedding);
   m.def("embed_fwd", &embed_fwd, py::arg("idx"), py::arg("weight"), py::arg("pos_weight") = py::none(),
         py::arg("positions") = py::none(), py::arg("scale") = 1.0, py::arg("start") = 0, py::arg("shard") = false);
   m.def("embed_grad", &embed_grad, py::arg("dy"), py::arg("idx"), py::arg("rows"), py::arg("scale") = 1.0,

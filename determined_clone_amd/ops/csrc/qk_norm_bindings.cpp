@@ -3,6 +3,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 
+#include "autograd_util.h"
 #include "qk_norm_api.h"
 
 namespace {
@@ -135,10 +136,60 @@ std::vector<Tensor> qk_norm_rope_bwd(const Tensor& dyq, const Tensor& dyk, const
                         partial.defined() ? partial.data_ptr<float>() : nullptr, to, stream());
   return {dq, dk, dw[0], dw[1]};
 }
+
+Tensor f32(const Tensor& w) { return w.defined() ? w.to(at::kFloat).contiguous() : w; }
+OptT opt(const Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
+Tensor viewable(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+// The operator with its gradient (an autograd node here: see EmbeddingNode).
+struct QkNormRopeNode : torch::autograd::Function<QkNormRopeNode> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q_in,
+                                                const Tensor& k_in, const OptT& wq, const OptT& wk, const OptT& cos,
+                                                const OptT& sin, int64_t rot, const OptT& positions, double eps) {
+    const Tensor q = viewable(q_in), k = viewable(k_in);
+    const Tensor none, w[2] = {given(wq) ? *wq : none, given(wk) ? *wk : none};
+    ctx->save_for_backward({q, k, w[0], w[1], given(cos) ? *cos : none, given(sin) ? *sin : none,
+                            given(positions) ? *positions : none});
+    // the parameters themselves, for their persistent gradients
+    ctx->saved_data["wq"] = w[0];
+    ctx->saved_data["wk"] = w[1];
+    ctx->saved_data["rot"] = rot;
+    ctx->saved_data["eps"] = eps;
+    return qk_norm_rope(q, k, opt(f32(w[0])), opt(f32(w[1])), cos, sin, rot, positions, eps);
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor params[2] = {ctx->saved_data["wq"].toTensor(), ctx->saved_data["wk"].toTensor()};
+    bool need[2];
+    OptT acc[2];
+    for (int i = 0; i < 2; ++i) {
+      need[i] = params[i].defined() && ctx->needs_input_grad(2 + i);
+      if (need[i]) acc[i] = dca::grad_target(params[i]);
+    }
+    auto d = qk_norm_rope_bwd(viewable(grads[0]), viewable(grads[1]), s[0], s[1], opt(f32(s[2])), opt(f32(s[3])),
+                              opt(s[4]), opt(s[5]), ctx->saved_data["rot"].toInt(), opt(s[6]),
+                              ctx->saved_data["eps"].toDouble(), need[0], need[1], acc[0], acc[1], OptT(), OptT());
+    torch::autograd::variable_list out(9);
+    for (int i = 0; i < 2; ++i) {
+      out[i] = d[i];
+      if (d[2 + i].defined()) out[2 + i] = d[2 + i].to(params[i].scalar_type());
+    }
+    return dca::once(std::move(out), grads[grads[0].requires_grad() ? 0 : 1]);
+  }
+};
+
+std::vector<Tensor> qk_norm_rope_autograd(const Tensor& q, const Tensor& k, const OptT& wq, const OptT& wk,
+                                          const OptT& cos, const OptT& sin, int64_t rot, const OptT& positions,
+                                          double eps) {
+  return QkNormRopeNode::apply(q, k, wq, wk, cos, sin, rot, positions, eps);
+}
 }  // namespace
 
 void register_qk_norm_ops(pybind11::module& m) {
   namespace py = pybind11;
+  m.def("qk_norm_rope_autograd", &qk_norm_rope_autograd);
   m.def("qk_norm_rope", &qk_norm_rope, py::arg("q"), py::arg("k"), py::arg("q_weight"), py::arg("k_weight"),
         py::arg("cos"), py::arg("sin"), py::arg("rot"), py::arg("positions"), py::arg("eps"));
   m.def("qk_norm_rope_bwd", &qk_norm_rope_bwd, py::arg("dyq"), py::arg("dyk"), py::arg("q"), py::arg("k"),

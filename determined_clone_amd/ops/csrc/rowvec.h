@@ -26,6 +26,24 @@ __device__ __forceinline__ void stv(void* base, int64_t elem, const RawVec<T, V>
   *reinterpret_cast<RawVec<T, V>*>(reinterpret_cast<typename T::raw*>(base) + elem) = r;
 }
 
+// Streamed forms, for data past the caches that is not read again soon.
+template <typename T, int V>
+__device__ __forceinline__ RawVec<T, V> ldv_nt(const void* base, int64_t elem) {
+  if constexpr (V * kElem<T> == 16)
+    return ldnt16(reinterpret_cast<const typename T::raw*>(base) + elem);
+  else
+    return ldv<T, V>(base, elem);
+}
+__device__ __forceinline__ void stnt16(void* p, const uint4& v) {
+  const dca_u32x4 r = {v.x, v.y, v.z, v.w};
+  __builtin_nontemporal_store(r, static_cast<dca_u32x4*>(p));
+}
+template <typename T, int V>
+__device__ __forceinline__ void stv_nt(void* base, int64_t elem, const RawVec<T, V>& r) {
+  if constexpr (V * kElem<T> == 16) stnt16(reinterpret_cast<typename T::raw*>(base) + elem, r);
+  else stv<T, V>(base, elem, r);
+}
+
 template <typename T, int V>
 __device__ __forceinline__ void unpackv(const RawVec<T, V>& r, float (&v)[V]) {
   if constexpr (std::is_same<T, F32>::value) {

@@ -13,9 +13,8 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
-from determined_clone_amd.ops import _ext, _grad
+from determined_clone_amd.ops import _ext
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -36,42 +35,6 @@ def reference_embedding(idx, weight, pos_weight=None, positions=None, scale=1.0,
         else:
             out = out + F.embedding(positions.long(), pos_weight).to(wide)
     return out.to(weight.dtype)
-
-
-def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return t if t is None or t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
-
-
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, idx, weight, pos_weight, positions, scale, vocab_start):
-        ctx.save_for_backward(idx, positions)
-        ctx.params = (weight, pos_weight)
-        ctx.scale, ctx.start = scale, vocab_start or 0
-        return _ext.load().embed_fwd(idx, _rows(weight.detach()),
-                                     None if pos_weight is None else _rows(pos_weight.detach()),
-                                     positions, scale, ctx.start, vocab_start is not None)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        C = _ext.load()
-        idx, positions = ctx.saved_tensors
-        weight, pos_weight = ctx.params
-        dw = dp = None
-        dy = dy.contiguous()
-        if ctx.needs_input_grad[1]:
-            acc = _grad.target(weight)
-            dw = C.embed_grad(dy, idx, weight.shape[0], ctx.scale, ctx.start, acc)
-            dw = None if acc is not None else dw
-        if ctx.needs_input_grad[2]:
-            acc = _grad.target(pos_weight)
-            if positions is None:
-                dp = C.embed_pos_grad(dy, pos_weight.shape[0], acc)
-            else:
-                dp = C.embed_grad(dy, positions, pos_weight.shape[0], 1.0, 0, acc)
-            dp = None if acc is not None else dp
-        return None, dw, dp, None, None, None
 
 
 def _check_index(t: torch.Tensor, what: str) -> None:
@@ -97,6 +60,8 @@ def embedding(idx: torch.Tensor, weight: torch.Tensor, pos_weight: Optional[torc
     _check_index(idx, "idx")
     if weight.dim() != 2 or not weight.is_floating_point():
         raise ValueError("embedding: weight must be a floating-point [V, E] table")
+    if vocab_start is not None and vocab_start < 0:
+        raise ValueError(f"embedding: vocab_start must not be negative, got {vocab_start}")
     if idx.device != weight.device:
         raise ValueError(f"embedding: idx on {idx.device}, weight on {weight.device}")
     if positions is not None and pos_weight is None:
@@ -111,15 +76,16 @@ def embedding(idx: torch.Tensor, weight: torch.Tensor, pos_weight: Optional[torc
             _check_index(positions, "positions")
             if positions.device != weight.device:
                 raise ValueError(f"embedding: positions on {positions.device}, weight on {weight.device}")
-            positions = positions.expand(idx.shape)  # raises for shapes that do not broadcast
+            if positions.shape != idx.shape:
+                positions = positions.expand(idx.shape)  # raises for shapes that do not broadcast
         elif idx.dim() == 0:
             raise ValueError("embedding: a single id needs its position")
         elif idx.shape[-1] > pos_weight.shape[0]:
             raise ValueError(f"embedding: {idx.shape[-1]} tokens, {pos_weight.shape[0]} positions")
     if not weight.is_cuda or weight.dtype not in _DTYPES:  # float64 tables: plain PyTorch
         return reference_embedding(idx, weight, pos_weight, positions, scale, vocab_start)
-    return _Embedding.apply(idx.contiguous(), weight, pos_weight,
-                            None if positions is None else positions.contiguous(), float(scale), vocab_start)
+    return _ext.load().embedding(idx, weight, pos_weight, positions, float(scale), vocab_start or 0,
+                                 vocab_start is not None)
 
 
 __all__ = ["embedding", "reference_embedding"]

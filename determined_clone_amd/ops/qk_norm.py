@@ -91,38 +91,6 @@ def _check(q, k, q_weight, k_weight, cos, sin, rot_dim, positions):
     return cos, sin, rot, positions
 
 
-def _gpu_view(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-class _QKNormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, rot, positions, eps):
-        q, k = _gpu_view(q), _gpu_view(k)
-        yq, yk = _ext.load().qk_norm_rope(q, k, _f32(q_weight), _f32(k_weight), cos, sin, rot, positions, eps)
-        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.rot, ctx.eps, ctx.params = rot, eps, (q_weight, k_weight)
-        return yq, yk
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dyq, dyk):
-        dq, dk, dwq, dwk = _backward(ctx, _gpu_view(dyq), _gpu_view(dyk), ctx.needs_input_grad[2:4])
-        return dq, dk, dwq, dwk, None, None, None, None, None
-
-
-def _backward(ctx, dyq, dyk, need, dq_out=None, dk_out=None):
-    """(dq, dk, dwq, dwk) from the context's q, k, weights, tables; weight gradients are added in
-    place (None) where the parameter has a persistent ``.grad``."""
-    q, k, wq, wk, cos, sin, positions = ctx.saved_tensors[:7]
-    acc = [_grad.target(p) if n else None for p, n in zip(ctx.params, need)]
-    dq, dk, dwq, dwk = _ext.load().qk_norm_rope_bwd(
-        dyq, dyk, q, k, _f32(wq), _f32(wk), cos, sin, ctx.rot, positions, ctx.eps, need[0], need[1],
-        acc[0], acc[1], dq_out, dk_out)
-    dw = [None if d is None else d.to(p.dtype) for d, p in ((dwq, wq), (dwk, wk))]
-    return dq, dk, dw[0], dw[1]
-
-
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
                  k_weight: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
                  sin: Optional[torch.Tensor] = None, rot_dim: Optional[int] = None,
@@ -143,7 +111,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
         return reference_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, rot, positions, eps)
     if q.dtype not in _DTYPES:
         raise ValueError(f"qk_norm_rope: GPU path needs bf16, fp16 or fp32, got {q.dtype}")
-    return _QKNormRope.apply(q, k, q_weight, k_weight, cos, sin, rot, positions, float(eps))
+    return tuple(_ext.load().qk_norm_rope_autograd(q, k, q_weight, k_weight, cos, sin, rot, positions, float(eps)))
 
 
 class _QKNormAttention(torch.autograd.Function):
@@ -165,12 +133,17 @@ class _QKNormAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        qkv, yq, yk, o, lse, kv_len = ctx.saved_tensors[7:]
+        C = _ext.load()
+        q, k, wq, wk, cos, sin, positions, qkv, yq, yk, o, lse, kv_len = ctx.saved_tensors
         dqkv = torch.empty_like(qkv)
         dq, dk, dv = dqkv.unbind(2)
-        _ext.load().attn_bwd(do, yq, yk, qkv[:, :, 2], o, lse, ctx.scale, ctx.causal, dq, dk, dv, kv_len)
-        _, _, dwq, dwk = _backward(ctx, dq, dk, ctx.needs_input_grad[1:3], dq, dk)
-        return (dqkv, dwq, dwk) + (None,) * 8
+        C.attn_bwd(do, yq, yk, qkv[:, :, 2], o, lse, ctx.scale, ctx.causal, dq, dk, dv, kv_len)
+        need = ctx.needs_input_grad[1:3]
+        acc = [_grad.target(p) if n else None for p, n in zip(ctx.params, need)]
+        _, _, dwq, dwk = C.qk_norm_rope_bwd(dq, dk, q, k, _f32(wq), _f32(wk), cos, sin, ctx.rot, positions,
+                                            ctx.eps, need[0], need[1], acc[0], acc[1], dq, dk)
+        dw = tuple(None if d is None else d.to(p.dtype) for d, p in zip((dwq, dwk), ctx.params))
+        return (dqkv,) + dw + (None,) * 8
 
 
 def qk_norm_attention_qkvpacked(qkv: torch.Tensor, q_weight: Optional[torch.Tensor] = None,

@@ -256,3 +256,7 @@ def test_refusals():
     assert g.shape == t.shape
     with pytest.raises(RuntimeError):
         g.sum().backward()  # no second derivatives
+    dy = torch.randn(2, 3, 4, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(embedding(idx, t), t, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        (g.sum() + dy.sum()).backward()
