@@ -25,50 +25,77 @@ constexpr int kFwdUnroll = 4;
 // Outputs past the L2s are streamed (67 MB: 20.2 against 22.1 us), smaller ones stay for their reader.
 constexpr int64_t kStreamBytes = 32 << 20;
 
-template <typename T, int V>
+// Several entries of an index array: their loads leave together.
+template <int N>
+__device__ __forceinline__ void read_index(const Index& a, int64_t first, const unsigned (&r)[N], int64_t (&out)[N]) {
+  if (a.is32) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) out[u] = static_cast<const int32_t*>(a.p)[first + r[u]];
+  } else {
+#pragma unroll
+    for (int u = 0; u < N; ++u) out[u] = static_cast<const int64_t*>(a.p)[first + r[u]];
+  }
+}
+
+// A workgroup takes a few rows, vector after vector. All ids of an unrolled step are read, then all
+// rows, with mistakes and the end of the stretch replaced by rows that exist: no load waits for
+// another of its kind.
+template <typename T, bool kAligned>
 __global__ __launch_bounds__(kFwdBlock) void embed_fwd_kernel(
     EmbedIds ids, const void* __restrict__ table, int64_t stride, EmbedPos pos, float scale,
     void* __restrict__ out, int E, int rows_per_block, bool stream) {
-  const unsigned nv = static_cast<unsigned>(E / V);
+  constexpr int V = kFull<T>;
+  const unsigned nv = static_cast<unsigned>((E + V - 1) / V);
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * rows_per_block;
   const int64_t left = ids.n - t0;
   const unsigned n = static_cast<unsigned>(left < rows_per_block ? left : rows_per_block) * nv;
   for (unsigned i0 = threadIdx.x; i0 < n; i0 += kFwdBlock * kFwdUnroll) {
-    RawVec<T, V> w[kFwdUnroll], p[kFwdUnroll];
-    bool wok[kFwdUnroll], pok[kFwdUnroll];
+    unsigned r[kFwdUnroll], c[kFwdUnroll];
+    int64_t id[kFwdUnroll], at[kFwdUnroll];
+    uint4 w[kFwdUnroll], p[kFwdUnroll];
 #pragma unroll
     for (int u = 0; u < kFwdUnroll; ++u) {
-      const unsigned i = i0 + u * kFwdBlock;
-      wok[u] = pok[u] = false;
-      if (i >= n) continue;
-      const unsigned r = i / nv;
-      const int64_t c = static_cast<int64_t>(i - r * nv) * V, t = t0 + r;
-      const int64_t id = ids.ids.at(t) - ids.start;
-      wok[u] = static_cast<uint64_t>(id) < static_cast<uint64_t>(ids.rows);
-      if (wok[u]) w[u] = ldv<T, V>(table, id * stride + c);
-      if (pos.rows) {
-        const int64_t at = pos.ids.p ? pos.ids.at(t) : t % pos.S;
-        pok[u] = static_cast<uint64_t>(at) < static_cast<uint64_t>(pos.rows);
-        if (pok[u]) p[u] = ldv<T, V>(pos.table, at * pos.stride + c);
+      const unsigned i = i0 + u * kFwdBlock < n ? i0 + u * kFwdBlock : n - 1;
+      r[u] = i / nv;
+      c[u] = (i - r[u] * nv) * V;
+    }
+    read_index(ids.ids, t0, r, id);
+    if (pos.rows) {
+      if (pos.ids.p) {
+        read_index(pos.ids, t0, r, at);
+      } else {
+#pragma unroll
+        for (int u = 0; u < kFwdUnroll; ++u)
+          at[u] = static_cast<uint32_t>(t0 + r[u]) % static_cast<uint32_t>(pos.S);
       }
     }
 #pragma unroll
     for (int u = 0; u < kFwdUnroll; ++u) {
-      const unsigned i = i0 + u * kFwdBlock;
-      if (i >= n) continue;
-      float a[V], b[V];
-      const float none = ids.shard ? 0.f : __builtin_nanf("");
-      if (wok[u]) unpackv<T, V>(w[u], a);
+      id[u] -= ids.start;
+      if (static_cast<uint64_t>(id[u]) >= static_cast<uint64_t>(ids.rows)) id[u] = -1;
+      w[u] = load_row<T, kAligned, false>(table, (id[u] < 0 ? 0 : id[u]) * stride + c[u], E - c[u]);
+    }
+    if (pos.rows) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) a[k] = wok[u] ? a[k] * scale : none;
-      if (pos.rows) {
-        if (pok[u]) unpackv<T, V>(p[u], b);
-#pragma unroll
-        for (int k = 0; k < V; ++k) a[k] = pok[u] ? a[k] + b[k] : __builtin_nanf("");
+      for (int u = 0; u < kFwdUnroll; ++u) {
+        if (static_cast<uint64_t>(at[u]) >= static_cast<uint64_t>(pos.rows)) at[u] = -1;
+        p[u] = load_row<T, kAligned, false>(pos.table, (at[u] < 0 ? 0 : at[u]) * pos.stride + c[u], E - c[u]);
       }
-      const int64_t to = t0 * E + static_cast<int64_t>(i) * V;
-      if (stream) stv_nt<T, V>(out, to, packv<T, V>(a));
-      else stv<T, V>(out, to, packv<T, V>(a));
+    }
+#pragma unroll
+    for (int u = 0; u < kFwdUnroll; ++u) {
+      if (i0 + u * kFwdBlock >= n) break;
+      float a[V], b[V];
+      unpackv<T, V>(w[u], a);
+      const float none = ids.shard ? 0.f : __builtin_nanf("");
+#pragma unroll
+      for (int k = 0; k < V; ++k) a[k] = id[u] < 0 ? none : a[k] * scale;
+      if (pos.rows) {
+        unpackv<T, V>(p[u], b);
+#pragma unroll
+        for (int k = 0; k < V; ++k) a[k] = at[u] < 0 ? __builtin_nanf("") : a[k] + b[k];
+      }
+      store_row<T, kAligned>(out, (t0 + r[u]) * E + c[u], E - c[u], packv<T, V>(a), stream);
     }
   }
 }
@@ -85,7 +112,7 @@ constexpr int kList = 256;
 // since their lines do not push each other's out of the caches half-written.
 __device__ __forceinline__ void zero_fill(void* p, int64_t bytes, int64_t first, int64_t step) {
   const int64_t n = bytes / 16;
-  for (int64_t i = first; i < n; i += step) stnt16(static_cast<uint4*>(p) + i, make_uint4(0, 0, 0, 0));
+  for (int64_t i = first; i < n; i += step) store_row<F32, true>(p, i * 4, 4, make_uint4(0, 0, 0, 0), true);
   if (first < bytes % 16) static_cast<char*>(p)[n * 16 + first] = 0;
 }
 
@@ -239,23 +266,24 @@ __global__ __launch_bounds__(kWaves * 64) void embed_place_kernel(const I* __res
 __device__ __forceinline__ int64_t partial_stride(int E) { return (E + 3) & ~3; }
 
 // out = scale a, or scale a + old
-template <typename T, int V>
-__device__ __forceinline__ void grad_store(void* out, int64_t at, float (&a)[V], float scale, bool accumulate,
-                                           const RawVec<T, V>& old) {
-  float o[V];
-  unpackv<T, V>(old, o);
+template <typename T, bool kAligned>
+__device__ __forceinline__ void grad_store(void* out, int64_t at, int64_t left, float (&a)[kFull<T>], float scale,
+                                           bool accumulate, const uint4& old) {
+  float o[kFull<T>];
+  unpackv<T, kFull<T>>(old, o);
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
+  for (int k = 0; k < kFull<T>; ++k) {
     a[k] *= scale;
     if (accumulate) a[k] += o[k];
   }
-  stv<T, V>(out, at, packv<T, V>(a));
+  store_row<T, kAligned>(out, at, left, packv<T, kFull<T>>(a), false);
 }
-template <typename T, int V>
-__device__ __forceinline__ void grad_store(void* out, int64_t at, float (&a)[V], float scale, bool accumulate) {
-  RawVec<T, V> old{};
-  if (accumulate) old = ldv<T, V>(out, at);
-  grad_store<T, V>(out, at, a, scale, accumulate, old);
+template <typename T, bool kAligned>
+__device__ __forceinline__ void grad_store(void* out, int64_t at, int64_t left, float (&a)[kFull<T>], float scale,
+                                           bool accumulate) {
+  uint4 old = make_uint4(0, 0, 0, 0);
+  if (accumulate) old = load_row<T, kAligned, false>(out, at, left);
+  grad_store<T, kAligned>(out, at, left, a, scale, accumulate, old);
 }
 
 // Few ids: a wave per table row and stretch of 64 V columns. Rows without an id are cleared (or left
@@ -263,9 +291,10 @@ __device__ __forceinline__ void grad_store(void* out, int64_t at, float (&a)[V],
 constexpr int kDirectIds = 512;
 constexpr int kDirectWaves = 4;
 constexpr int kDirectUnroll = 8;
-template <typename T, int V>
+template <typename T, bool kAligned>
 __global__ __launch_bounds__(kDirectWaves * 64) void embed_grad_direct_kernel(
     EmbedIds ids, const void* __restrict__ dy, void* __restrict__ out, int E, float scale, bool accumulate) {
+  constexpr int V = kFull<T>;
   const int lane = threadIdx.x & 63;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kDirectWaves + (threadIdx.x >> 6);
   if (row >= ids.rows) return;
@@ -281,14 +310,14 @@ __global__ __launch_bounds__(kDirectWaves * 64) void embed_grad_direct_kernel(
     uint64_t own = __ballot(i0 + lane < n && ids.ids.at(i0 + lane) - ids.start == row);
     any |= own != 0;
     while (own) {
-      RawVec<T, V> r[kDirectUnroll];
+      uint4 r[kDirectUnroll];
       int got = 0;
 #pragma unroll
       for (int u = 0; u < kDirectUnroll; ++u) {
         if (!own) break;
         const int t = i0 + __builtin_ctzll(own);
         own &= own - 1;
-        if (ok) r[u] = ldv<T, V>(dy, static_cast<int64_t>(t) * E + c);
+        if (ok) r[u] = load_row<T, kAligned, false>(dy, static_cast<int64_t>(t) * E + c, E - c);
         ++got;
       }
 #pragma unroll
@@ -301,7 +330,7 @@ __global__ __launch_bounds__(kDirectWaves * 64) void embed_grad_direct_kernel(
       }
     }
   }
-  if (ok && (any || !accumulate)) grad_store<T, V>(out, row * E + c, a, scale, accumulate);
+  if (ok && (any || !accumulate)) grad_store<T, kAligned>(out, row * E + c, E - c, a, scale, accumulate);
 }
 
 // Workgroup x takes sorted entries [x K, (x + 1) K), K <= 64, workgroup y a stretch of columns. Every
@@ -311,11 +340,12 @@ __global__ __launch_bounds__(kDirectWaves * 64) void embed_grad_direct_kernel(
 // sum of a token that began in an earlier range (its "head"), 1 of one that began here and goes on
 // (its "tail").
 constexpr int kGradUnroll = 8;
-template <typename T, int V, bool kAdd>
+template <typename T, bool kAligned, bool kAdd>
 __global__ __launch_bounds__(256) void embed_grad_kernel(const uint64_t* __restrict__ sorted,
                                                          const void* __restrict__ dy, void* out,
                                                          float* __restrict__ partial, int64_t n, int E, int K,
                                                          float scale) {
+  constexpr int V = kFull<T>;
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
   const bool ok = c < E;
   const int64_t lo = static_cast<int64_t>(blockIdx.x) * K;
@@ -334,24 +364,28 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const uint64_t* __restr
 #pragma unroll
   for (int k = 0; k < V; ++k) a[k] = 0.f;
   struct Batch {
-    RawVec<T, V> dy[kGradUnroll], old[kAdd ? kGradUnroll : 1];
+    uint4 dy[kGradUnroll], old[kAdd ? kGradUnroll : 1];
   };
+  // no branches around the rows' loads, so that a wait for one batch leaves the next one in flight:
+  // past the end the last entry's row again, lanes past E (their vectors' values are not used) column 0
+  const int col = ok ? c : 0;
   auto load = [&](Batch& r, int e) {
 #pragma unroll
     for (int u = 0; u < kGradUnroll; ++u) {
-      if (e + u >= cnt) break;
       const uint32_t tok = __builtin_amdgcn_readlane(tok_l, e + u);
-      if (ok && row_at(e + u) >= 0) r.dy[u] = ldv_nt<T, V>(dy, static_cast<int64_t>(tok) * E + c);
-      if constexpr (kAdd) {
+      r.dy[u] = load_row<T, kAligned, true>(dy, static_cast<int64_t>(tok) * E + col, E - col);
+    }
+    if constexpr (kAdd) {
+#pragma unroll
+      for (int u = 0; u < kGradUnroll; ++u) {
+        if (e + u >= cnt) break;
         const int row = row_at(e + u);
-        if (ok && row >= 0 && row != row_at(e + u + 1)) r.old[u] = ldv<T, V>(out, static_cast<int64_t>(row) * E + c);
+        if (ok && row >= 0 && row != row_at(e + u + 1))
+          r.old[u] = load_row<T, kAligned, false>(out, static_cast<int64_t>(row) * E + c, E - c);
       }
     }
   };
-  Batch now, then;
-  load(now, 0);
-  for (int e = 0; e < cnt; e += kGradUnroll) {
-    if (e + kGradUnroll < cnt) load(then, e + kGradUnroll);
+  auto add = [&](const Batch& now, int e) {
 #pragma unroll
     for (int u = 0; u < kGradUnroll; ++u) {
       if (e + u >= cnt) break;
@@ -373,17 +407,27 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const uint64_t* __restr
         if (open || !ends) {
           float* to = open ? head : head + ps;
 #pragma unroll
-          for (int k = 0; k < V; ++k) to[c + k] = a[k];
+          for (int k = 0; k < V; ++k)
+            if (kAligned || c + k < E) to[c + k] = a[k];
         } else {
-          grad_store<T, V>(out, static_cast<int64_t>(row) * E + c, a, scale, kAdd, now.old[kAdd ? u : 0]);
+          grad_store<T, kAligned>(out, static_cast<int64_t>(row) * E + c, E - c, a, scale, kAdd,
+                                  now.old[kAdd ? u : 0]);
         }
       }
 #pragma unroll
       for (int k = 0; k < V; ++k) a[k] = 0.f;
       open = false;
     }
+  };
+  Batch now, then;
+  load(now, 0);
+  int e = 0;
+  for (; e + kGradUnroll < cnt; e += kGradUnroll) {
+    load(then, e + kGradUnroll);
+    add(now, e);
     now = then;
   }
+  add(now, e);
 }
 
 // Joins the tokens that cross ranges: the workgroup in whose range a token begins adds the heads of
@@ -433,8 +477,8 @@ __global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(const uint6
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     if (c + k >= E) break;
-    float one[1] = {v[k]};
-    grad_store<T, 1>(out, static_cast<int64_t>(row) * E + c + k, one, scale, accumulate);
+    const int64_t at = static_cast<int64_t>(row) * E + c + k;
+    Elem<T>::put(out, at, accumulate ? v[k] * scale + Elem<T>::get(out, at) : v[k] * scale);
   }
 }
 
@@ -442,9 +486,10 @@ __global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(const uint6
 // Column sums of dy [B][N]: a lane takes V columns, the workgroup's waves split the batch and join
 // in a fixed order.
 constexpr int kSumUnroll = 8;
-template <typename T, int V>
+template <typename T, bool kAligned>
 __global__ __launch_bounds__(1024) void batch_sum_kernel(const void* __restrict__ dy, void* __restrict__ out,
                                                          int64_t B, int64_t N, bool accumulate) {
+  constexpr int V = kFull<T>;
   extern __shared__ float red[];  // [waves][64][V]
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int64_t c = (static_cast<int64_t>(blockIdx.x) * 64 + lane) * V;
@@ -452,19 +497,24 @@ __global__ __launch_bounds__(1024) void batch_sum_kernel(const void* __restrict_
 #pragma unroll
   for (int k = 0; k < V; ++k) a[k] = 0.f;
   if (c < N) {
-    for (int64_t b = w; b < B; b += static_cast<int64_t>(waves) * kSumUnroll) {
-      RawVec<T, V> r[kSumUnroll];
+    int64_t b = w;
+    for (; b + (kSumUnroll - 1) * waves < B; b += static_cast<int64_t>(waves) * kSumUnroll) {
+      uint4 r[kSumUnroll];
 #pragma unroll
-      for (int u = 0; u < kSumUnroll; ++u)
-        if (b + u * waves < B) r[u] = ldv<T, V>(dy, (b + u * waves) * N + c);
+      for (int u = 0; u < kSumUnroll; ++u) r[u] = load_row<T, kAligned, false>(dy, (b + u * waves) * N + c, N - c);
 #pragma unroll
       for (int u = 0; u < kSumUnroll; ++u) {
-        if (b + u * waves >= B) continue;
         float x[V];
         unpackv<T, V>(r[u], x);
 #pragma unroll
         for (int k = 0; k < V; ++k) a[k] += x[k];
       }
+    }
+    for (; b < B; b += waves) {
+      float x[V];
+      unpackv<T, V>(load_row<T, kAligned, false>(dy, b * N + c, N - c), x);
+#pragma unroll
+      for (int k = 0; k < V; ++k) a[k] += x[k];
     }
   }
   if (waves > 1) {
@@ -476,15 +526,20 @@ __global__ __launch_bounds__(1024) void batch_sum_kernel(const void* __restrict_
 #pragma unroll
       for (int k = 0; k < V; ++k) a[k] += red[(i * 64 + lane) * V + k];
   }
-  if (c < N) grad_store<T, V>(out, c, a, 1.f, accumulate);
+  if (c < N) grad_store<T, kAligned>(out, c, N - c, a, 1.f, accumulate);
 }
 
+template <typename T, typename F>
+void dispatch_a(bool aligned, F&& f) {
+  if (aligned) f(T{}, BTag<true>{});
+  else f(T{}, BTag<false>{});
+}
 template <typename F>
-void dispatch_tv(TDtype dt, int vec_bytes, F&& f) {
+void dispatch_ta(TDtype dt, bool aligned, F&& f) {
   switch (dt) {
-    case TDtype::kBF16: dispatch_v<BF16>(vec_bytes, f); break;
-    case TDtype::kF16: dispatch_v<F16>(vec_bytes, f); break;
-    default: dispatch_v<F32>(vec_bytes, f); break;
+    case TDtype::kBF16: dispatch_a<BF16>(aligned, f); break;
+    case TDtype::kF16: dispatch_a<F16>(aligned, f); break;
+    default: dispatch_a<F32>(aligned, f); break;
   }
 }
 
@@ -498,18 +553,19 @@ int64_t partial_floats(int64_t n, int E) {
 }
 }  // namespace
 
-void embed_fwd(TDtype dt, int vec_bytes, const EmbedIds& ids, const void* table, int64_t stride,
+void embed_fwd(TDtype dt, bool aligned, const EmbedIds& ids, const void* table, int64_t stride,
                const EmbedPos& pos, float scale, void* out, int E, hipStream_t st) {
   if (ids.n == 0 || E == 0) return;
-  dispatch_tv(dt, vec_bytes, [&](auto t, auto v) {
+  dispatch_ta(dt, aligned, [&](auto t, auto a) {
     using T = decltype(t);
-    constexpr int V = decltype(v)::value;
-    const int64_t nv = E / V;
+    constexpr int V = kFull<T>;
+    constexpr bool A = decltype(a)::value;
+    const int64_t nv = (E + V - 1) / V;
     // one pass of the workgroup's unrolled loop, as long as that leaves 1024 workgroups
     int64_t r = kFwdBlock * kFwdUnroll / nv;
     if (r > ids.n / 1024) r = ids.n / 1024;
     if (r < 1) r = 1;
-    hipLaunchKernelGGL((embed_fwd_kernel<T, V>), dim3(static_cast<unsigned>((ids.n + r - 1) / r)),
+    hipLaunchKernelGGL((embed_fwd_kernel<T, A>), dim3(static_cast<unsigned>((ids.n + r - 1) / r)),
                        dim3(kFwdBlock), 0, st, ids, table, stride, pos, scale, out, E, static_cast<int>(r),
                        ids.n * E * kElem<T> >= kStreamBytes);
   });
@@ -539,15 +595,16 @@ static void place(const EmbedIds& ids, uint64_t* sorted, void* clear, int64_t cl
   else place<I, 1024, 8>(ids, shift, sorted, clear, clear_bytes, st);
 }
 
-void embed_grad(TDtype dt, int vec_bytes, const EmbedIds& ids, const void* dy, void* out, int E,
+void embed_grad(TDtype dt, bool aligned, const EmbedIds& ids, const void* dy, void* out, int E,
                 float scale, bool accumulate, void* workspace, hipStream_t st) {
   const int64_t n = ids.n;
   if (E == 0 || ids.rows == 0) return;
   if (n <= kDirectIds) {
-    dispatch_tv(dt, vec_bytes, [&](auto t, auto v) {
+    dispatch_ta(dt, aligned, [&](auto t, auto a) {
       using T = decltype(t);
-      constexpr int V = decltype(v)::value;
-      hipLaunchKernelGGL((embed_grad_direct_kernel<T, V>),
+      constexpr int V = kFull<T>;
+      constexpr bool A = decltype(a)::value;
+      hipLaunchKernelGGL((embed_grad_direct_kernel<T, A>),
                          dim3(static_cast<unsigned>((ids.rows + kDirectWaves - 1) / kDirectWaves),
                               static_cast<unsigned>((E + 64 * V - 1) / (64 * V))),
                          dim3(kDirectWaves * 64), 0, st, ids, dy, out, E, scale, accumulate);
@@ -561,17 +618,18 @@ void embed_grad(TDtype dt, int vec_bytes, const EmbedIds& ids, const void* dy, v
   else place<int64_t>(ids, sorted, out, clear, st);
   const int K = grad_range(n);
   const unsigned nb = static_cast<unsigned>((n + K - 1) / K);
-  dispatch_tv(dt, vec_bytes, [&](auto t, auto v) {
+  dispatch_ta(dt, aligned, [&](auto t, auto a) {
     using T = decltype(t);
-    constexpr int V = decltype(v)::value;
-    const int nv = E / V;
+    constexpr int V = kFull<T>;
+    constexpr bool A = decltype(a)::value;
+    const int nv = (E + V - 1) / V;
     const int threads = nv >= 256 ? 256 : (nv + 63) / 64 * 64;
     const dim3 grid(nb, static_cast<unsigned>((nv + threads - 1) / threads));
     if (accumulate)
-      hipLaunchKernelGGL((embed_grad_kernel<T, V, true>), grid, dim3(threads), 0, st, sorted, dy, out, partial,
+      hipLaunchKernelGGL((embed_grad_kernel<T, A, true>), grid, dim3(threads), 0, st, sorted, dy, out, partial,
                          n, E, K, scale);
     else
-      hipLaunchKernelGGL((embed_grad_kernel<T, V, false>), grid, dim3(threads), 0, st, sorted, dy, out, partial,
+      hipLaunchKernelGGL((embed_grad_kernel<T, A, false>), grid, dim3(threads), 0, st, sorted, dy, out, partial,
                          n, E, K, scale);
     if (nb > 1)
       hipLaunchKernelGGL(embed_join_kernel<T>, dim3(nb, static_cast<unsigned>((E + 255) / 256)),
@@ -579,16 +637,17 @@ void embed_grad(TDtype dt, int vec_bytes, const EmbedIds& ids, const void* dy, v
   });
 }
 
-void batch_sum(TDtype dt, int vec_bytes, const void* dy, void* out, int64_t B, int64_t N,
+void batch_sum(TDtype dt, bool aligned, const void* dy, void* out, int64_t B, int64_t N,
                bool accumulate, hipStream_t st) {
   if (N == 0) return;
-  dispatch_tv(dt, vec_bytes, [&](auto t, auto v) {
+  dispatch_ta(dt, aligned, [&](auto t, auto a) {
     using T = decltype(t);
-    constexpr int V = decltype(v)::value;
-    const int64_t tiles = (N / V + 63) / 64;
+    constexpr int V = kFull<T>;
+    constexpr bool A = decltype(a)::value;
+    const int64_t tiles = (N + 64 * V - 1) / (64 * V);
     int waves = 1;  // split the batch where the columns alone do not fill the chip
     while (waves < 16 && waves * 2 <= B && tiles * waves < 4096) waves *= 2;
-    hipLaunchKernelGGL((batch_sum_kernel<T, V>), dim3(static_cast<unsigned>(tiles)), dim3(waves * 64),
+    hipLaunchKernelGGL((batch_sum_kernel<T, A>), dim3(static_cast<unsigned>(tiles)), dim3(waves * 64),
                        waves > 1 ? static_cast<size_t>(waves) * 64 * V * sizeof(float) : 0, st, dy, out, B, N,
                        accumulate);
   });

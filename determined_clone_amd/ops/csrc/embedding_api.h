@@ -7,6 +7,7 @@
 #include "transformer_api.h"
 
 namespace dca {
+// `aligned`: all addresses and row lengths are multiples of 16 bytes.
 // Token ids -> table rows: row = id - start; `shard`: ids outside [start, start + rows) belong to
 // another shard (zero rows), otherwise they are mistakes (NaN rows).
 struct EmbedIds {
@@ -24,16 +25,16 @@ struct EmbedPos {
   Index ids;
   int64_t S = 1;
 };
-void embed_fwd(TDtype dt, int vec_bytes, const EmbedIds& ids, const void* table, int64_t stride,
+void embed_fwd(TDtype dt, bool aligned, const EmbedIds& ids, const void* table, int64_t stride,
                const EmbedPos& pos, float scale, void* out, int E, hipStream_t st);
 // bytes of workspace embed_grad needs for n ids and rows of E
 int64_t embed_grad_workspace(int64_t n, int E);
 // out[row] = scale * sum of dy's rows with that id, zero for rows without one; `accumulate`: added to
 // what is there, rows without an id untouched. dy [n][E], out [rows][E] (16-byte aligned unless
 // accumulating), both contiguous.
-void embed_grad(TDtype dt, int vec_bytes, const EmbedIds& ids, const void* dy, void* out, int E,
+void embed_grad(TDtype dt, bool aligned, const EmbedIds& ids, const void* dy, void* out, int E,
                 float scale, bool accumulate, void* workspace, hipStream_t st);
 // out[j] (+)= sum_b dy[b][j] for dy [B][N]
-void batch_sum(TDtype dt, int vec_bytes, const void* dy, void* out, int64_t B, int64_t N,
+void batch_sum(TDtype dt, bool aligned, const void* dy, void* out, int64_t B, int64_t N,
                bool accumulate, hipStream_t st);
 }  // namespace dca

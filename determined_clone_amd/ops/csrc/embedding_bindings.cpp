@@ -13,6 +13,7 @@ using torch::Tensor;
 using OptT = c10::optional<Tensor>;
 
 hipStream_t stream() { return at::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream(); }
+constexpr int64_t kMaxWidth = 1 << 20;  // the kernels' grids take a row's columns in their second dimension
 bool given(const OptT& t) { return t.has_value() && t->defined(); }
 
 dca::TDtype tdt(const Tensor& t) {
@@ -39,7 +40,7 @@ dca::EmbedIds ids_of(const Tensor& idx, const Tensor& like, int64_t rows, int64_
 void check_table(const Tensor& t, const char* what) {
   TORCH_CHECK(t.is_cuda() && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1), what,
               ": a GPU table [rows, E] with contiguous rows is required");
-  TORCH_CHECK(t.size(1) < std::numeric_limits<int32_t>::max(), what, ": rows too long");
+  TORCH_CHECK(t.size(1) <= kMaxWidth, what, ": rows of more than ", kMaxWidth, " elements");
 }
 
 // idx [...], weight [V, E], pos_weight [P, E], positions like idx (absent: t % seq) -> [..., E]
@@ -74,9 +75,10 @@ Tensor embed_fwd(const Tensor& idx, const Tensor& weight, const OptT& pos_weight
       TORCH_CHECK(idx.dim() > 0 && idx.size(-1) <= pos.rows, "embed_fwd: more tokens than positions");
       pos.S = idx.size(-1);
     }
-    TORCH_CHECK(pos.rows > 0 || idx.numel() == 0, "embed_fwd: empty position table");
   }
-  dca::embed_fwd(tdt(weight), vec.bytes(), ids, weight.data_ptr(), weight.stride(0), pos,
+  TORCH_CHECK(idx.numel() == 0 || (weight.size(0) > 0 && (!given(pos_weight) || pos.rows > 0)),
+              "embed_fwd: ids for an empty table");
+  dca::embed_fwd(tdt(weight), vec.bytes() == 16, ids, weight.data_ptr(), weight.stride(0), pos,
                  static_cast<float>(scale), out.data_ptr(), static_cast<int>(E), stream());
   return out;
 }
@@ -98,6 +100,7 @@ Tensor embed_grad(const Tensor& dy_in, const Tensor& idx, int64_t rows, double s
   const c10::DeviceGuard g(dy_in.device());
   Tensor dy = dy_in.contiguous();
   const int64_t E = dy.size(-1);
+  TORCH_CHECK(E <= kMaxWidth, "embed_grad: rows of more than ", kMaxWidth, " elements");
   const dca::EmbedIds ids = ids_of(idx, dy, rows, start, true);
   Tensor out = destination(acc, rows, E, dy);
   if (E == 0) return out;
@@ -106,7 +109,7 @@ Tensor embed_grad(const Tensor& dy_in, const Tensor& idx, int64_t rows, double s
   vec.elems(E);
   vec.ptr(dy.data_ptr());
   vec.ptr(out.data_ptr());
-  dca::embed_grad(tdt(dy), vec.bytes(), ids, dy.data_ptr(), out.data_ptr(), static_cast<int>(E),
+  dca::embed_grad(tdt(dy), vec.bytes() == 16, ids, dy.data_ptr(), out.data_ptr(), static_cast<int>(E),
                   static_cast<float>(scale), given(acc), ws.data_ptr(), stream());
   return out;
 }
@@ -126,7 +129,7 @@ Tensor embed_pos_grad(const Tensor& dy_in, int64_t rows, const OptT& acc) {
   vec.elems(N);
   vec.ptr(dy.data_ptr());
   vec.ptr(out.data_ptr());
-  dca::batch_sum(tdt(dy), vec.bytes(), dy.data_ptr(), out.data_ptr(), dy.numel() / N, N, given(acc), stream());
+  dca::batch_sum(tdt(dy), vec.bytes() == 16, dy.data_ptr(), out.data_ptr(), dy.numel() / N, N, given(acc), stream());
   return out;
 }
 

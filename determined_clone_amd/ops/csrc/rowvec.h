@@ -1,7 +1,5 @@
-// Row vectors of 16, 4 or 2 bytes for kernels that take any width and alignment: V elements of
-// storage type T, loaded raw (so that unrolled loads are all in flight before the first use) and
-// unpacked to fp32. The host picks the widest V that divides the row length, the row strides and
-// the base addresses (widest_vec).
+// Vectors of a storage type T for kernels that take any width and alignment: loaded raw (so that
+// unrolled loads are all in flight before the first use) and unpacked to fp32.
 #pragma once
 #include "common.h"
 
@@ -26,22 +24,56 @@ __device__ __forceinline__ void stv(void* base, int64_t elem, const RawVec<T, V>
   *reinterpret_cast<RawVec<T, V>*>(reinterpret_cast<typename T::raw*>(base) + elem) = r;
 }
 
-// Streamed forms, for data past the caches that is not read again soon.
-template <typename T, int V>
-__device__ __forceinline__ RawVec<T, V> ldv_nt(const void* base, int64_t elem) {
-  if constexpr (V * kElem<T> == 16)
-    return ldnt16(reinterpret_cast<const typename T::raw*>(base) + elem);
-  else
-    return ldv<T, V>(base, elem);
+// 16-byte vectors of rows of any length and alignment. kAligned: all addresses are multiples of 16
+// and `left`, the elements from `elem` to the row's end, is a multiple of the vector's; otherwise the
+// address is a multiple of the element's (gfx950 takes such loads and stores as they are) and a row's
+// last vector goes element by element, zeros behind it. kStream: past the caches, for data that is
+// not read again soon.
+template <int kBytes> struct LooseVec;
+typedef dca_u32x4 dca_u32x4_2 __attribute__((aligned(2)));
+typedef dca_u32x4 dca_u32x4_4 __attribute__((aligned(4)));
+template <> struct LooseVec<2> { using type = dca_u32x4_2; };
+template <> struct LooseVec<4> { using type = dca_u32x4_4; };
+template <typename T, bool kAligned>
+using RowPtr = std::conditional_t<kAligned, dca_u32x4, typename LooseVec<kElem<T>>::type>;
+
+template <typename T, bool kAligned, bool kStream>
+__device__ __forceinline__ uint4 load_row(const void* base, int64_t elem, int64_t left) {
+  const auto* p = reinterpret_cast<const typename T::raw*>(base) + elem;
+  if (kAligned || left >= kFull<T>) {
+    const auto* q = reinterpret_cast<const RowPtr<T, kAligned>*>(p);
+    dca_u32x4 v;
+    if constexpr (kStream) v = __builtin_nontemporal_load(q);
+    else v = *q;
+    return make_uint4(v.x, v.y, v.z, v.w);
+  }
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < kFull<T>; ++i) {
+    if (i >= left) break;
+    if constexpr (kElem<T> == 2) w[i / 2] |= static_cast<uint32_t>(p[i]) << (i % 2 * 16);
+    else w[i] = __float_as_uint(p[i]);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ void stnt16(void* p, const uint4& v) {
-  const dca_u32x4 r = {v.x, v.y, v.z, v.w};
-  __builtin_nontemporal_store(r, static_cast<dca_u32x4*>(p));
-}
-template <typename T, int V>
-__device__ __forceinline__ void stv_nt(void* base, int64_t elem, const RawVec<T, V>& r) {
-  if constexpr (V * kElem<T> == 16) stnt16(reinterpret_cast<typename T::raw*>(base) + elem, r);
-  else stv<T, V>(base, elem, r);
+
+template <typename T, bool kAligned>
+__device__ __forceinline__ void store_row(void* base, int64_t elem, int64_t left, const uint4& r, bool stream) {
+  auto* p = reinterpret_cast<typename T::raw*>(base) + elem;
+  if (kAligned || left >= kFull<T>) {
+    auto* q = reinterpret_cast<RowPtr<T, kAligned>*>(p);
+    const dca_u32x4 v = {r.x, r.y, r.z, r.w};
+    if (stream) __builtin_nontemporal_store(v, q);
+    else *q = v;
+    return;
+  }
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < kFull<T>; ++i) {
+    if (i >= left) break;
+    if constexpr (kElem<T> == 2) p[i] = static_cast<uint16_t>(w[i / 2] >> (i % 2 * 16));
+    else p[i] = __uint_as_float(w[i]);
+  }
 }
 
 template <typename T, int V>
@@ -100,6 +132,10 @@ struct WidestVec {
   int bytes() const { return bits % 16 == 0 ? 16 : (bits % 4 == 0 ? 4 : elem); }
 };
 
+template <bool B>
+struct BTag {
+  static constexpr bool value = B;
+};
 template <int V>
 struct VTag {
   static constexpr int value = V;
