@@ -22,7 +22,7 @@ namespace {
 // ------------------------------------------------------------------ forward
 constexpr int kFwdBlock = 256;
 constexpr int kFwdUnroll = 4;
-// Outputs past the L2s are streamed (67 MB: 20.2 against 22.1 us), smaller ones stay for their reader.
+// Outputs past the L2s are streamed (203 MB: 57 against 66 us), smaller ones stay for their reader.
 constexpr int64_t kStreamBytes = 32 << 20;
 
 // Several entries of an index array: their loads leave together.
@@ -40,10 +40,10 @@ __device__ __forceinline__ void read_index(const Index& a, int64_t first, const 
 // A workgroup takes a few rows, vector after vector. All ids of an unrolled step are read, then all
 // rows, with mistakes and the end of the stretch replaced by rows that exist: no load waits for
 // another of its kind.
-template <typename T, bool kAligned>
+template <typename T, bool kAligned, bool kStream>
 __global__ __launch_bounds__(kFwdBlock) void embed_fwd_kernel(
     EmbedIds ids, const void* __restrict__ table, int64_t stride, EmbedPos pos, float scale,
-    void* __restrict__ out, int E, int rows_per_block, bool stream) {
+    void* __restrict__ out, int E, int rows_per_block) {
   constexpr int V = kFull<T>;
   const unsigned nv = static_cast<unsigned>((E + V - 1) / V);
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * rows_per_block;
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(kFwdBlock) void embed_fwd_kernel(
 #pragma unroll
         for (int k = 0; k < V; ++k) a[k] = at[u] < 0 ? __builtin_nanf("") : a[k] + b[k];
       }
-      store_row<T, kAligned>(out, (t0 + r[u]) * E + c[u], E - c[u], packv<T, V>(a), stream);
+      store_row<T, kAligned, kStream>(out, (t0 + r[u]) * E + c[u], E - c[u], packv<T, V>(a));
     }
   }
 }
@@ -107,14 +107,16 @@ __device__ __forceinline__ int row_of(uint64_t entry) { return static_cast<int>(
 constexpr int kPlaceUnroll = 8;
 constexpr int kList = 256;
 
-// 16 bytes of zeros at a time, the last bytes one by one; `p` is 16-byte aligned. Streamed, and dy read
-// that way by the kernels that follow: 31x2047 tokens, E = 1600, fp16: 180 against 217 us altogether,
-// since their lines do not push each other's out of the caches half-written.
+// 16 bytes of zeros at a time, the last bytes one by one; `p` is 16-byte aligned. Not streamed: that
+// measured 34 against 28 us beside the sort (161 MB).
 __device__ __forceinline__ void zero_fill(void* p, int64_t bytes, int64_t first, int64_t step) {
   const int64_t n = bytes / 16;
-  for (int64_t i = first; i < n; i += step) store_row<F32, true>(p, i * 4, 4, make_uint4(0, 0, 0, 0), true);
+  for (int64_t i = first; i < n; i += step) store_row<F32, true, false>(p, i * 4, 4, make_uint4(0, 0, 0, 0));
   if (first < bytes % 16) static_cast<char*>(p)[n * 16 + first] = 0;
 }
+
+// A wave's own LDS accesses are carried out in the order they are issued: the compiler keeps it.
+__device__ __forceinline__ void keep_order() { asm volatile("" ::: "memory"); }
 
 // Workgroups [0, 2^shift): the sort; b owns the ids with b in their low bits, rows r with r mod 2^shift
 // = b and, behind them, the ids that have no row (counter kRows - 1). The others clear `clear`
@@ -147,9 +149,8 @@ __global__ __launch_bounds__(kWaves * 64) void embed_place_kernel(const I* __res
   // steps of 64 ids for a wave, a multiple of the unrolled loops' (what is past n counts nowhere)
   const int64_t steps = (n + kThreads * kPlaceUnroll - 1) / (kThreads * kPlaceUnroll) * kPlaceUnroll;
   const int64_t lo = w * steps * 64;
-  volatile uint32_t* mine = count + w * kRows;  // volatile: a wave's own reads and writes stay in order
 #pragma unroll
-  for (int i = 0; i < kRows / 64; ++i) mine[i * 64 + lane] = 0;
+  for (int i = 0; i < kRows / 64; ++i) count[w * kRows + i * 64 + lane] = 0;
   const uint64_t lower = (1ull << lane) - 1;
   uint32_t below = 0;
   int64_t listed = 0;
@@ -232,8 +233,10 @@ __global__ __launch_bounds__(kWaves * 64) void embed_place_kernel(const I* __res
       if (rest) same = left;
     }
     if (own) {
-      const uint32_t before = static_cast<uint32_t>(__popcll(same & lower)), to = mine[d];
-      if (before == 0) mine[d] = to + static_cast<uint32_t>(__popcll(same));
+      const uint32_t before = static_cast<uint32_t>(__popcll(same & lower)), to = count[w * kRows + d];
+      keep_order();
+      if (before == 0) count[w * kRows + d] = to + static_cast<uint32_t>(__popcll(same));
+      keep_order();
       const uint32_t row = d == kRows - 1u ? ~0u : d << shift | me;
       sorted[to + before] = static_cast<uint64_t>(row) << 32 | static_cast<uint32_t>(at);
     }
@@ -276,7 +279,7 @@ __device__ __forceinline__ void grad_store(void* out, int64_t at, int64_t left, 
     a[k] *= scale;
     if (accumulate) a[k] += o[k];
   }
-  store_row<T, kAligned>(out, at, left, packv<T, kFull<T>>(a), false);
+  store_row<T, kAligned, false>(out, at, left, packv<T, kFull<T>>(a));
 }
 template <typename T, bool kAligned>
 __device__ __forceinline__ void grad_store(void* out, int64_t at, int64_t left, float (&a)[kFull<T>], float scale,
@@ -565,9 +568,9 @@ void embed_fwd(TDtype dt, bool aligned, const EmbedIds& ids, const void* table, 
     int64_t r = kFwdBlock * kFwdUnroll / nv;
     if (r > ids.n / 1024) r = ids.n / 1024;
     if (r < 1) r = 1;
-    hipLaunchKernelGGL((embed_fwd_kernel<T, A>), dim3(static_cast<unsigned>((ids.n + r - 1) / r)),
-                       dim3(kFwdBlock), 0, st, ids, table, stride, pos, scale, out, E, static_cast<int>(r),
-                       ids.n * E * kElem<T> >= kStreamBytes);
+    auto* kernel = ids.n * E * kElem<T> >= kStreamBytes ? embed_fwd_kernel<T, A, true> : embed_fwd_kernel<T, A, false>;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((ids.n + r - 1) / r)), dim3(kFwdBlock), 0, st, ids, table,
+                       stride, pos, scale, out, E, static_cast<int>(r));
   });
 }
 

@@ -2,7 +2,9 @@
 //
 //   N = sqrt(sum g^2) | sum |g| | max |g|  over all tensors,   g *= min(1, max_norm / (N + 1e-6))
 //
-// Bound by HBM: the norm reads every gradient once, clipping reads and writes them once more. Tensors
+// Bound by HBM: the norm reads every gradient once, clipping reads and writes them once more. At 774M
+// elements in 436 tensors (GPT-2-large, bf16 and fp32, 1.55 GB) the norm takes 250 us (6.2 TB/s of
+// reads) and the scaling 495 us (6.3 TB/s). Tensors
 // are cut into chunks of one size, a workgroup a chunk, and up to kMaxTensors tensors go by value in
 // the arguments of one launch: no table to copy to the device, nothing to keep alive, graph-capturable.
 // Sums are held in 64 bits (gradients of 1e-25 or 1e+25 neither vanish nor overflow when squared, and
@@ -42,7 +44,8 @@ __device__ __forceinline__ Piece piece_of(const TensorTable& t, uint32_t x) {
     else hi = mid - 1;
   }
   Piece a;
-  a.p = reinterpret_cast<void*>(t.p[lo]);
+  // through the global address space: from a plain integer the compiler makes flat accesses
+  a.p = (void*)reinterpret_cast<__attribute__((address_space(1))) char*>(t.p[lo]);
   a.dt = static_cast<int>(t.n_dt[lo] & 3);
   const int64_t n = t.n_dt[lo] >> 2;
   a.lo = static_cast<int64_t>(x - t.first[lo]) * t.chunk;
@@ -90,16 +93,17 @@ __device__ __forceinline__ double block_join(double v, double* red) {
   return v;
 }
 
-template <NormKind kKind, typename T>
+template <NormKind kKind, typename T, bool kStream>
 __device__ __forceinline__ double piece_norm(const Piece& a) {
   double s[kUnroll] = {};
   walk<T>(
       a, [&](int64_t i) { float v[1]; unpackv<T, 1>(ldv<T, 1>(a.p, i), v); take<kKind>(s[0], v[0]); },
       [&](int64_t body, int64_t i, int64_t vecs) {
-        RawVec<T, kFull<T>> r[kUnroll];
+        uint4 r[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
-          if (i + u * kNormBlock < vecs) r[u] = ldv<T, kFull<T>>(a.p, body + (i + u * kNormBlock) * kFull<T>);
+          if (i + u * kNormBlock < vecs)
+            r[u] = load_row<T, true, kStream>(a.p, body + (i + u * kNormBlock) * kFull<T>, kFull<T>);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
           if (i + u * kNormBlock >= vecs) continue;
@@ -114,14 +118,14 @@ __device__ __forceinline__ double piece_norm(const Piece& a) {
   return s[0];
 }
 
-template <NormKind kKind>
+template <NormKind kKind, bool kStream>
 __global__ __launch_bounds__(kNormBlock) void norm_partial_kernel(TensorTable t, double* __restrict__ partial) {
   __shared__ double red[kNormBlock / 64];
   const Piece a = piece_of(t, blockIdx.x);
   double s;
-  if (a.dt == static_cast<int>(TDtype::kBF16)) s = piece_norm<kKind, BF16>(a);
-  else if (a.dt == static_cast<int>(TDtype::kF16)) s = piece_norm<kKind, F16>(a);
-  else s = piece_norm<kKind, F32>(a);
+  if (a.dt == static_cast<int>(TDtype::kBF16)) s = piece_norm<kKind, BF16, kStream>(a);
+  else if (a.dt == static_cast<int>(TDtype::kF16)) s = piece_norm<kKind, F16, kStream>(a);
+  else s = piece_norm<kKind, F32, kStream>(a);
   s = block_join<kKind>(s, red);
   if (threadIdx.x == 0) partial[t.partial0 + blockIdx.x] = s;
 }
@@ -136,7 +140,7 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(const double* __restric
   if (threadIdx.x == 0) norm[0] = static_cast<float>(kKind == NormKind::kL2 ? sqrt(s) : s);
 }
 
-template <typename T>
+template <typename T, bool kStream>
 __device__ __forceinline__ void piece_scale(const Piece& a, float c) {
   walk<T>(
       a,
@@ -147,10 +151,11 @@ __device__ __forceinline__ void piece_scale(const Piece& a, float c) {
         stv<T, 1>(a.p, i, packv<T, 1>(v));
       },
       [&](int64_t body, int64_t i, int64_t vecs) {
-        RawVec<T, kFull<T>> r[kUnroll];
+        uint4 r[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
-          if (i + u * kNormBlock < vecs) r[u] = ldv<T, kFull<T>>(a.p, body + (i + u * kNormBlock) * kFull<T>);
+          if (i + u * kNormBlock < vecs)
+            r[u] = load_row<T, true, kStream>(a.p, body + (i + u * kNormBlock) * kFull<T>, kFull<T>);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
           if (i + u * kNormBlock >= vecs) continue;
@@ -158,38 +163,48 @@ __device__ __forceinline__ void piece_scale(const Piece& a, float c) {
           unpackv<T, kFull<T>>(r[u], v);
 #pragma unroll
           for (int k = 0; k < kFull<T>; ++k) v[k] *= c;
-          stv<T, kFull<T>>(a.p, body + (i + u * kNormBlock) * kFull<T>, packv<T, kFull<T>>(v));
+          store_row<T, true, kStream>(a.p, body + (i + u * kNormBlock) * kFull<T>, kFull<T>, packv<T, kFull<T>>(v));
         }
       });
 }
 
 // The coefficient in the order of the formula, in fp32; a NaN norm makes every gradient NaN. A
 // gradient times 1 is itself, so workgroups of a list within the limit leave it alone.
+template <bool kStream>
 __global__ __launch_bounds__(kNormBlock) void clip_kernel(TensorTable t, const float* __restrict__ norm,
                                                           float max_norm) {
   const float c = max_norm / (norm[0] + 1e-6f);
   if (c >= 1.f) return;
   const Piece a = piece_of(t, blockIdx.x);
-  if (a.dt == static_cast<int>(TDtype::kBF16)) piece_scale<BF16>(a, c);
-  else if (a.dt == static_cast<int>(TDtype::kF16)) piece_scale<F16>(a, c);
-  else piece_scale<F32>(a, c);
+  if (a.dt == static_cast<int>(TDtype::kBF16)) piece_scale<BF16, kStream>(a, c);
+  else if (a.dt == static_cast<int>(TDtype::kF16)) piece_scale<F16, kStream>(a, c);
+  else piece_scale<F32, kStream>(a, c);
 }
 
-// Elements a workgroup takes: large lists 32k (the norm's partials stay few), small ones less, so
-// that there are workgroups for every CU.
-int64_t chunk_of(const std::vector<GradTensor>& t) {
-  int64_t total = 0;
-  for (const auto& x : t) total += x.n;
-  int64_t c = 2048;
+// How a list is walked. Lists that do not fit the 256 MB of last-level cache are streamed past it (774M
+// elements, bf16: norm 241 against 295 us, scaling 495 against 545 us); from smaller ones the scaling
+// finds in it what the norm has read.
+struct Walk {
+  int64_t norm_chunk;  // elements a workgroup takes: up to 32k, which keeps the norm's partials few
+  int64_t clip_chunk;  // the scaling has none to keep: 8k (the list above: 16k 520 us, 2k 515 us)
+  bool stream;
+};
+Walk walk_of(const std::vector<GradTensor>& t) {
+  int64_t total = 0, bytes = 0;
+  for (const auto& x : t) {
+    total += x.n;
+    bytes += x.n * (x.dt == TDtype::kF32 ? 4 : 2);
+  }
+  int64_t c = 2048;  // small lists: workgroups for every CU
   while (c < 32768 && total / c > 2048) c *= 2;
-  return c;
+  return {c, c < 8192 ? c : 8192, bytes > 256 << 20};
 }
 
 // f(table, workgroups) for every launch of the list
 template <typename F>
-void for_launches(const std::vector<GradTensor>& t, F&& f) {
+void for_launches(const std::vector<GradTensor>& t, int64_t chunk, F&& f) {
   TensorTable a;
-  a.chunk = chunk_of(t);
+  a.chunk = chunk;
   a.partial0 = 0;
   a.count = 0;
   uint32_t blocks = 0;
@@ -212,9 +227,11 @@ void for_launches(const std::vector<GradTensor>& t, F&& f) {
 
 template <NormKind kKind>
 void grad_norm_kind(const std::vector<GradTensor>& t, double* partial, float* norm, hipStream_t st) {
+  const Walk walk = walk_of(t);
   int64_t parts = 0;
-  for_launches(t, [&](const TensorTable& a, uint32_t blocks) {
-    hipLaunchKernelGGL(norm_partial_kernel<kKind>, dim3(blocks), dim3(kNormBlock), 0, st, a, partial);
+  for_launches(t, walk.norm_chunk, [&](const TensorTable& a, uint32_t blocks) {
+    auto* kernel = walk.stream ? norm_partial_kernel<kKind, true> : norm_partial_kernel<kKind, false>;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kNormBlock), 0, st, a, partial);
     parts += blocks;
   });
   hipLaunchKernelGGL(norm_join_kernel<kKind>, dim3(1), dim3(1024), 0, st, partial, parts, norm);
@@ -222,7 +239,7 @@ void grad_norm_kind(const std::vector<GradTensor>& t, double* partial, float* no
 }  // namespace
 
 int64_t grad_norm_workspace(const std::vector<GradTensor>& t) {
-  const int64_t c = chunk_of(t);
+  const int64_t c = walk_of(t).norm_chunk;
   int64_t n = 1;
   for (const auto& x : t) n += (x.n + c - 1) / c;
   return n;
@@ -235,8 +252,10 @@ void grad_norm(const std::vector<GradTensor>& t, NormKind kind, double* partial,
 }
 
 void grad_clip(const std::vector<GradTensor>& t, const float* norm, float max_norm, hipStream_t st) {
-  for_launches(t, [&](const TensorTable& a, uint32_t blocks) {
-    hipLaunchKernelGGL(clip_kernel, dim3(blocks), dim3(kNormBlock), 0, st, a, norm, max_norm);
+  const Walk walk = walk_of(t);
+  for_launches(t, walk.clip_chunk, [&](const TensorTable& a, uint32_t blocks) {
+    auto* kernel = walk.stream ? clip_kernel<true> : clip_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kNormBlock), 0, st, a, norm, max_norm);
   });
 }
 }  // namespace dca

@@ -57,13 +57,15 @@ __device__ __forceinline__ uint4 load_row(const void* base, int64_t elem, int64_
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <typename T, bool kAligned>
-__device__ __forceinline__ void store_row(void* base, int64_t elem, int64_t left, const uint4& r, bool stream) {
+// (kStream is a template argument also because the compiler would join the two kinds of store of a
+// branch into one plain store.)
+template <typename T, bool kAligned, bool kStream>
+__device__ __forceinline__ void store_row(void* base, int64_t elem, int64_t left, const uint4& r) {
   auto* p = reinterpret_cast<typename T::raw*>(base) + elem;
   if (kAligned || left >= kFull<T>) {
     auto* q = reinterpret_cast<RowPtr<T, kAligned>*>(p);
     const dca_u32x4 v = {r.x, r.y, r.z, r.w};
-    if (stream) __builtin_nontemporal_store(v, q);
+    if constexpr (kStream) __builtin_nontemporal_store(v, q);
     else *q = v;
     return;
   }
