@@ -3,8 +3,8 @@
 // Forward: out[t] = scale * W[id_t] + P[pos_t] in fp32, rounded once.
 //
 // Gradient: dW[v] = scale * sum_{t: id_t = v} dy[t], without float atomics, so that the result does
-// not depend on scheduling. Up to kDirectIds ids: a wave per table row looks through all ids and adds
-// the rows of those that are its own, in order. More ids are sorted by row (stably), and workgroups
+// not depend on scheduling. With few ids (direct()) a wave per table row looks through all of them and
+// adds the rows of those that are its own, in order. More ids are sorted by row (stably), and workgroups
 // take equal ranges of the SORTED order: a frequent token is spread over as many workgroups as its
 // rows need, a rare one costs one row. A token inside one range is written once; one that crosses
 // ranges leaves fp32 partial rows which a second kernel joins in order.
@@ -291,7 +291,6 @@ __device__ __forceinline__ void grad_store(void* out, int64_t at, int64_t left, 
 
 // Few ids: a wave per table row and stretch of 64 V columns. Rows without an id are cleared (or left
 // alone when adding), so that this is the gradient's only launch.
-constexpr int kDirectIds = 512;
 constexpr int kDirectWaves = 4;
 constexpr int kDirectUnroll = 8;
 template <typename T, bool kAligned>
@@ -339,9 +338,8 @@ __global__ __launch_bounds__(kDirectWaves * 64) void embed_grad_direct_kernel(
 // Workgroup x takes sorted entries [x K, (x + 1) K), K <= 64, workgroup y a stretch of columns. Every
 // wave holds the range's entries in its lanes, so all row addresses are known from the start; the
 // next rows' loads (and, when adding, of the table rows that end among them) leave before the present
-// ones are added. partial holds two rows a workgroup: 0 the
-// sum of a token that began in an earlier range (its "head"), 1 of one that began here and goes on
-// (its "tail").
+// ones are added. partial holds two rows a workgroup: 0 the sum of a token that began in an earlier
+// range (its "head"), 1 of one that began here and goes on (its "tail").
 constexpr int kGradUnroll = 8;
 template <typename T, bool kAligned, bool kAdd>
 __global__ __launch_bounds__(256) void embed_grad_kernel(const uint64_t* __restrict__ sorted,
@@ -550,6 +548,12 @@ void dispatch_ta(TDtype dt, bool aligned, F&& f) {
 // E = 1024, bf16, both kernels: 8 entries 42 us, 16 38 us, 32 33 us, 64 36 us).
 int grad_range(int64_t n) { return n >= 16384 ? 32 : (n >= 4096 ? 16 : 8); }
 
+// Whether a wave per table row is quicker than the sort and its two further launches. It looks through
+// n ids for every row, so the answer depends on both (kernels alone, ids spread out: 256 ids for 512 rows
+// of 128 fp32 9 against 12 us, 512 ids 14 against 13; 50304 rows of 1024 bf16, 128 ids 21 against 24,
+// 256 ids 28 against 23). All ids the same is the sort's better case: 256 of them 31 against 13 us.
+bool direct(int64_t n, int64_t rows) { return n <= 128 || (n <= 256 && rows <= 4096); }
+
 int64_t partial_floats(int64_t n, int E) {
   const int64_t K = grad_range(n);
   return (n + K - 1) / K * 2 * ((E + 3) & ~3);
@@ -575,8 +579,8 @@ void embed_fwd(TDtype dt, bool aligned, const EmbedIds& ids, const void* table, 
 }
 
 // The workspace: the sorted entries, the partial rows.
-int64_t embed_grad_workspace(int64_t n, int E) {
-  return n <= kDirectIds ? 0 : (n + 1) / 2 * 16 + partial_floats(n, E) * 4;
+int64_t embed_grad_workspace(int64_t n, int64_t rows, int E) {
+  return direct(n, rows) ? 0 : (n + 1) / 2 * 16 + partial_floats(n, E) * 4;
 }
 
 template <typename I, int kRows, int kWaves>
@@ -602,7 +606,7 @@ void embed_grad(TDtype dt, bool aligned, const EmbedIds& ids, const void* dy, vo
                 float scale, bool accumulate, void* workspace, hipStream_t st) {
   const int64_t n = ids.n;
   if (E == 0 || ids.rows == 0) return;
-  if (n <= kDirectIds) {
+  if (direct(n, ids.rows)) {
     dispatch_ta(dt, aligned, [&](auto t, auto a) {
       using T = decltype(t);
       constexpr int V = kFull<T>;

@@ -27,8 +27,8 @@ struct EmbedPos {
 };
 void embed_fwd(TDtype dt, bool aligned, const EmbedIds& ids, const void* table, int64_t stride,
                const EmbedPos& pos, float scale, void* out, int E, hipStream_t st);
-// bytes of workspace embed_grad needs for n ids and rows of E
-int64_t embed_grad_workspace(int64_t n, int E);
+// bytes of workspace embed_grad needs for n ids and a table of `rows` rows of E
+int64_t embed_grad_workspace(int64_t n, int64_t rows, int E);
 // out[row] = scale * sum of dy's rows with that id, zero for rows without one; `accumulate`: added to
 // what is there, rows without an id untouched. dy [n][E], out [rows][E] (16-byte aligned unless
 // accumulating), both contiguous.

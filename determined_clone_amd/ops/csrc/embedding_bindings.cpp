@@ -104,7 +104,7 @@ Tensor embed_grad(const Tensor& dy_in, const Tensor& idx, int64_t rows, double s
   const dca::EmbedIds ids = ids_of(idx, dy, rows, start, true);
   Tensor out = destination(acc, rows, E, dy);
   if (E == 0) return out;
-  Tensor ws = torch::empty({dca::embed_grad_workspace(ids.n, static_cast<int>(E))}, dy.options().dtype(at::kByte));
+  Tensor ws = torch::empty({dca::embed_grad_workspace(ids.n, ids.rows, static_cast<int>(E))}, dy.options().dtype(at::kByte));
   dca::WidestVec vec(static_cast<int>(dy.element_size()));
   vec.elems(E);
   vec.ptr(dy.data_ptr());

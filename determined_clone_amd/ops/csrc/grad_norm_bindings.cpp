@@ -35,8 +35,8 @@ bool describe(const std::vector<Tensor>& grads, bool write, std::vector<dca::Gra
   out.reserve(grads.size());
   for (const Tensor& g : grads) {
     if (!g.defined() || g.layout() != at::kStrided || !g.is_cuda() || g.device() != grads[0].device() ||
-        g.is_conj() || g.is_neg())
-      return false;
+        g.is_conj() || g.is_neg() || g.unsafeGetTensorImpl()->key_set().has(c10::DispatchKey::Python))
+      return false;  // (the last: tensor subclasses, which may have no memory of their own)
     dca::TDtype dt;
     switch (g.scalar_type()) {
       case at::kBFloat16: dt = dca::TDtype::kBF16; break;

@@ -83,15 +83,39 @@ def test_given_positions(dtype, integer):
     assert torch.equal(row[0], out[0])
 
 
-# n around the range, chunk (4096) and merge (16 chunks) borders; table rows around digit borders
-@pytest.mark.parametrize("n", [0, 1, 2, 63, 64, 65, 1000, 4095, 4096, 4097, 8192, 12289, 16384, 65536, 65537, 70001])
-def test_sorted_gradient_lengths(n):
-    idx, _, _, dy = _inputs(1, n, 5000, 8, torch.float32, seed=n)
-    dw = _ext.load().embed_grad(dy, idx, 5000)
-    _check_grad(dw, dy, idx, 5000)
+# n around the borders of the single-launch form (128, 256), ranges and walks; below, table rows around
+# the borders of the sort's owners (256) and counters (255, 1023 each)
+@pytest.mark.parametrize("rows", [700, 5000])
+@pytest.mark.parametrize("n", [0, 1, 2, 63, 64, 65, 128, 129, 256, 257, 1000, 4095, 4096, 4097, 8192, 12289, 16384, 65536, 65537, 70001])
+def test_sorted_gradient_lengths(n, rows):
+    idx, _, _, dy = _inputs(1, n, rows, 8, torch.float32, seed=n)
+    dw = _ext.load().embed_grad(dy, idx, rows)
+    _check_grad(dw, dy, idx, rows)
 
 
-@pytest.mark.parametrize("v", [1, 2, 255, 256, 257, 65535, 65536, 65537, 300000])
+@pytest.mark.parametrize("e", [8, 1000])
+@pytest.mark.parametrize("n", [200, 3000])
+def test_few_ids_with_a_row(n, e):
+    """Most ids belong to other shards, or to no table at all; the others are added to the old rows."""
+    idx, _, _, dy = _inputs(1, n, 5000, e, torch.bfloat16, seed=n)
+    idx[0, ::7] = -5
+    acc = torch.randn(40, e, device="cuda").bfloat16()
+    old = acc.clone()
+    _ext.load().embed_grad(dy, idx, 40, 0.5, 100, acc)
+    _check_grad(acc, dy, idx, 40, 0.5, old, start=100)
+    idx.fill_(-1)
+    assert not _ext.load().embed_grad(dy, idx, 40).any()
+
+
+def test_a_wide_vocabulary():
+    """More rows than 256 workgroups have counters for (1023 each)."""
+    v = 400_000
+    idx, _, _, dy = _inputs(1, 3000, v, 16, torch.float32, seed=11)
+    idx[0, :200] = v - 1
+    _check_grad(_ext.load().embed_grad(dy, idx, v), dy, idx, v)
+
+
+@pytest.mark.parametrize("v", [1, 2, 255, 256, 257, 65279, 65280, 65281, 65537, 261888, 261889])
 def test_sorted_gradient_table_sizes(v):
     idx, _, _, dy = _inputs(2, 5000, v, 8, torch.bfloat16, seed=v)
     idx[0, :3] = v - 1
