@@ -106,6 +106,7 @@ __device__ __forceinline__ int row_of(uint64_t entry) { return static_cast<int>(
 
 constexpr int kPlaceUnroll = 8;
 constexpr int kList = 256;
+constexpr int kCrowd = 8;
 
 // 16 bytes of zeros at a time, the last bytes one by one; `p` is 16-byte aligned. Not streamed: that
 // measured 34 against 28 us beside the sort (161 MB).
@@ -146,6 +147,28 @@ __global__ __launch_bounds__(kWaves * 64) void embed_place_kernel(const I* __res
     const int64_t row = static_cast<int64_t>(id) - start;
     return static_cast<uint64_t>(row) < static_cast<uint64_t>(rows) ? static_cast<uint32_t>(row) >> shift : kRows - 1u;
   };
+  // of the lanes in `own`, those with this lane's counter: one counter at a time, and bit by bit where
+  // there are many
+  auto peers = [&](uint64_t own, uint32_t d) {
+    uint64_t left = own, same = 0;
+    const bool in = own >> lane & 1;
+    for (int k = 0; k < 3 && left; ++k) {
+      const uint32_t one = __builtin_amdgcn_readlane(d, __builtin_ctzll(left));
+      const uint64_t s = __builtin_amdgcn_ballot_w64(in && d == one);
+      if (s >> lane & 1) same = s;
+      left &= ~s;
+    }
+    if (left) {
+      const bool rest = left >> lane & 1;
+      for (int b = 0; (kRows >> b) > 1; ++b) {
+        const bool one = (d >> b) & 1;
+        const uint64_t v = __builtin_amdgcn_ballot_w64(one);
+        left &= one ? v : ~v;
+      }
+      if (rest) same = left;
+    }
+    return same;
+  };
   // steps of 64 ids for a wave, a multiple of the unrolled loops' (what is past n counts nowhere)
   const int64_t steps = (n + kThreads * kPlaceUnroll - 1) / (kThreads * kPlaceUnroll) * kPlaceUnroll;
   const int64_t lo = w * steps * 64;
@@ -174,9 +197,12 @@ __global__ __launch_bounds__(kWaves * 64) void embed_place_kernel(const I* __res
       const bool own = owner == me;
       const uint64_t all = __builtin_amdgcn_ballot_w64(own);
       if (!all) continue;
+      const uint32_t d = counter_of(id[u]);
+      // many at once are mostly of one counter, where their additions would wait for each other
+      const uint64_t same = __popcll(all) > kCrowd ? peers(all, d) : 0;
       if (own) {
-        const uint32_t d = counter_of(id[u]);
-        atomicAdd(&count[w * kRows + d], 1u);
+        if (!same) atomicAdd(&count[w * kRows + d], 1u);
+        else if (!(same & lower)) atomicAdd(&count[w * kRows + d], static_cast<uint32_t>(__popcll(same)));
         const int64_t at = listed + __popcll(all & lower);
         if (at < kList) list[w][at] = d << 22 | static_cast<uint32_t>((j + u) * 64 + lane);
       }
@@ -215,23 +241,7 @@ __global__ __launch_bounds__(kWaves * 64) void embed_place_kernel(const I* __res
   __syncthreads();
   // places the lanes' own ids, `d` their counters, `at` their indexes
   auto put = [&](bool own, uint32_t d, int64_t at) {
-    uint64_t left = __builtin_amdgcn_ballot_w64(own), same = 0;
-    // lanes with the same counter: one at a time, and bit by bit where there are many
-    for (int k = 0; k < 3 && left; ++k) {
-      const uint32_t one = __builtin_amdgcn_readlane(d, __builtin_ctzll(left));
-      const uint64_t s = __builtin_amdgcn_ballot_w64(own && d == one);
-      if (s >> lane & 1) same = s;
-      left &= ~s;
-    }
-    if (left) {
-      const bool rest = left >> lane & 1;
-      for (int b = 0; (kRows >> b) > 1; ++b) {
-        const bool one = (d >> b) & 1;
-        const uint64_t v = __builtin_amdgcn_ballot_w64(one);
-        left &= one ? v : ~v;
-      }
-      if (rest) same = left;
-    }
+    const uint64_t same = peers(__builtin_amdgcn_ballot_w64(own), d);
     if (own) {
       const uint32_t before = static_cast<uint32_t>(__popcll(same & lower)), to = count[w * kRows + d];
       keep_order();
@@ -446,14 +456,16 @@ __global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(const uint6
   const int before = row_of(sorted[lo > 0 ? lo - 1 : 0]);
   if (row < 0 || next != row) return;                   // ends here
   if (lo > 0 && first == row && before == row) return;  // began earlier
-  // the last range that begins with the token: 64 ranges a step, since a step costs a trip to memory
+  // the last range that begins with the token (they follow each other): 64 ranges a step, since a step
+  // costs a trip to memory, 64 times as far apart while all have it, and back
   const int64_t x = blockIdx.x, nb = (n + K - 1) / K;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int64_t last = x;
-  for (uint64_t with = ~0ull; with == ~0ull;) {
-    const int64_t at = last + 1 + lane;
-    with = __builtin_amdgcn_ballot_w64(at < nb && row_of(sorted[at < nb ? at * K : 0]) == row);
-    last += __popcll(with);  // the ranges that begin with it follow each other
+  for (int64_t apart = 1; apart;) {
+    const int64_t at = last + (lane + 1) * apart;
+    const int with = __popcll(__builtin_amdgcn_ballot_w64(at < nb && row_of(sorted[at < nb ? at * K : 0]) == row));
+    last += with * apart;
+    apart = with == 64 ? apart * 64 : apart / 64;
   }
   const int c = (blockIdx.y * 64 + lane) * 4;
   const int64_t ps = partial_stride(E);
