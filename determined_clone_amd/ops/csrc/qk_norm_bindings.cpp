@@ -164,8 +164,9 @@ struct QkNormRopeNode : torch::autograd::Function<QkNormRopeNode> {
     const Tensor params[2] = {ctx->saved_data["wq"].toTensor(), ctx->saved_data["wk"].toTensor()};
     bool need[2];
     OptT acc[2];
+    size_t edge = 2;  // needs_input_grad counts the graph's edges: q, k and the weights that are there
     for (int i = 0; i < 2; ++i) {
-      need[i] = params[i].defined() && ctx->needs_input_grad(2 + i);
+      need[i] = params[i].defined() && ctx->needs_input_grad(edge++);
       if (need[i]) acc[i] = dca::grad_target(params[i]);
     }
     auto d = qk_norm_rope_bwd(viewable(grads[0]), viewable(grads[1]), s[0], s[1], opt(f32(s[2])), opt(f32(s[3])),

@@ -113,6 +113,40 @@ def test_low_precision_weights(w_dtype):
     _case(2, 30, 4, 4, 64, 64, torch.bfloat16, w_dtype=w_dtype)
 
 
+@pytest.mark.parametrize("rot", [0, 32])
+@pytest.mark.parametrize("trained", ["q", "k"])
+@pytest.mark.parametrize("other", ["absent", "frozen"])
+@pytest.mark.parametrize("persistent", [False, True])
+def test_one_trained_weight(rot, trained, other, persistent):
+    """The gradient of one weight, the other one absent or frozen, returned or added to ``.grad``."""
+    g = torch.Generator(device="cuda").manual_seed(rot)
+    q = torch.randn(2, 21, 4, 64, generator=g, device="cuda")
+    k = torch.randn(2, 21, 2, 64, generator=g, device="cuda")
+    dy = [torch.randn(x.shape, generator=g, device="cuda") for x in (q, k)]
+    w = torch.nn.Parameter(torch.rand(64, generator=g, device="cuda") + 0.5)
+    frozen = torch.rand(64, generator=g, device="cuda") + 0.5 if other == "frozen" else None
+    cos, sin = T.rope_tables(21, rot, device="cuda") if rot else (None, None)
+    which = "qk".index(trained)
+    ws = (w, frozen) if which == 0 else (frozen, w)
+    old = torch.randn(64, generator=g, device="cuda")
+    if persistent:
+        w._dca_direct_grad = True
+        w.grad = old.clone()
+    leaves = [x.requires_grad_(True) for x in (q, k)]
+    y = qk_norm_rope(*leaves, *ws, cos, sin, rot_dim=rot, eps=1e-5)
+    torch.autograd.backward(y, dy)
+    for i in range(2):
+        _check(leaves[i], ws[i], dy[i], cos, sin, rot, None, 1e-5, y[i].detach(), leaves[i].grad,
+               None if i != which or persistent else w.grad)
+    if persistent:
+        plain = w.grad.double() - old.double()
+        w.grad, w._dca_direct_grad = None, False
+        torch.autograd.backward(qk_norm_rope(q.detach(), k.detach(), *ws, cos, sin, rot_dim=rot, eps=1e-5)[which],
+                                dy[which])
+        # the same sum with one more fp32 addition
+        assert ((plain - w.grad.double()).abs() <= U * (old.double().abs() + w.grad.double().abs()) * 1.001).all()
+
+
 def test_no_tokens_and_no_key_heads():
     w = torch.ones(64, device="cuda", requires_grad=True)
     q = torch.randn(2, 0, 4, 64, device="cuda", requires_grad=True)
