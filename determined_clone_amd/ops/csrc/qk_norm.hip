@@ -413,7 +413,16 @@ void qk_norm_rope_bwd(TDtype dt, int vec_bytes, const QkShape& s, const HeadView
     });
   }
   if (!want || s.D == 0) return;
-  hipLaunchKernelGGL(qk_dw_kernel, dim3((2 * s.D + kSumCols - 1) / kSumCols), dim3(1024), 0, st, partial, rows, s.D,
-                     dw[0] ? *dw[0] : ColumnOut{}, dw[1] ? *dw[1] : ColumnOut{});
+  auto sum = [&](const ColumnOut& q, const ColumnOut& k) {
+    hipLaunchKernelGGL(qk_dw_kernel, dim3((2 * s.D + kSumCols - 1) / kSumCols), dim3(1024), 0, st, partial, rows, s.D, q,
+                       k);
+  };
+  const ColumnOut q = dw[0] ? *dw[0] : ColumnOut{}, k = dw[1] ? *dw[1] : ColumnOut{};
+  if (q.p0 && q.p0 == k.p0) {  // one weight for both, added to its gradient: one after the other
+    sum(q, ColumnOut{});
+    sum(ColumnOut{}, k);
+  } else {
+    sum(q, k);
+  }
 }
 }  // namespace dca

@@ -237,6 +237,35 @@ def test_accumulates_into_persistent_grads(dtype):
         torch.testing.assert_close(w.grad, p + 1, rtol=2 * torch.finfo(dtype).eps, atol=torch.finfo(dtype).eps)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("packed", [False, True])
+def test_one_weight_for_queries_and_keys(dtype, packed):
+    """Both of its gradients arrive in the one persistent ``.grad``, each addition rounded once to it."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    qkv = torch.randn(2, 70, 3, 4, 64, generator=g, device="cuda").bfloat16()
+    dy = torch.randn(2, 70, 4, 64, generator=g, device="cuda").bfloat16()
+    w = torch.nn.Parameter((torch.rand(64, generator=g, device="cuda") + 0.5).to(dtype))
+
+    def backward(wq, wk):
+        if packed:
+            qk_norm_attention_qkvpacked(qkv, wq, wk).backward(dy)
+        else:
+            torch.autograd.backward(qk_norm_rope(qkv[:, :, 0], qkv[:, :, 1], wq, wk), (dy, dy))
+
+    parts = [w.detach().float().requires_grad_(True) for _ in range(2)]  # the two gradients by themselves
+    backward(*parts)
+    a, b = (p.grad.double() for p in parts)
+    w._dca_direct_grad = True
+    w.grad = torch.randn(64, generator=g, device="cuda").to(dtype)
+    old = w.grad.double()
+    backward(w, w)
+    # two additions in fp32 and their roundings to the type, half a step of each sum
+    step = torch.finfo(dtype).eps / 2 + U
+    first = old + a
+    bound = step * (first.abs() + (first + b).abs()) * (1 + step) ** 2
+    assert ((w.grad.double() - (first + b)).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("rot", [0, 16, 64])
 def test_packed_attention(rot):
     """The fused function against its parts: the same kernels in the same order, bit for bit."""
