@@ -16,10 +16,10 @@ inline c10::optional<torch::Tensor> grad_target(const torch::Tensor& p) {
   return t.cast<torch::Tensor>();
 }
 
-// `out`, gradients that cannot be differentiated again: under create_graph, with an incoming gradient
-// `dy` that could be, doing so raises.
-inline torch::autograd::variable_list once(torch::autograd::variable_list&& out, const torch::Tensor& dy) {
-  if (!at::GradMode::is_enabled() || !dy.requires_grad()) return std::move(out);
+// `out`, gradients that cannot be differentiated again: under create_graph doing so raises. `depends`:
+// whether they depend on anything that could ask for it (an incoming gradient, saved inputs).
+inline torch::autograd::variable_list once(torch::autograd::variable_list&& out, bool depends) {
+  if (!at::GradMode::is_enabled() || !depends) return std::move(out);
   for (auto& g : out)
     if (g.defined()) g = g.detach().set_requires_grad(true);
   auto node = std::make_shared<torch::autograd::DelayedError>(

@@ -170,7 +170,7 @@ struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
                                             : embed_pos_grad(dy, pos_weight.size(0), acc);
       if (!given(acc)) out[2] = dp;
     }
-    return dca::once(std::move(out), grads[0]);
+    return dca::once(std::move(out), grads[0].requires_grad());  // linear: the tables do not enter
   }
 
  private:

@@ -177,7 +177,7 @@ struct QkNormRopeNode : torch::autograd::Function<QkNormRopeNode> {
       out[i] = d[i];
       if (d[2 + i].defined()) out[2 + i] = d[2 + i].to(params[i].scalar_type());
     }
-    return dca::once(std::move(out), grads[grads[0].requires_grad() ? 0 : 1]);
+    return dca::once(std::move(out), true);  // they depend on q, k and the weights
   }
 };
 

@@ -10,7 +10,6 @@ import math
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from determined_clone_amd.ops import _ext, _grad
 from determined_clone_amd.ops.transformer import _attn_gpu_ok, _f32, _kv_len, reference_attention
@@ -114,6 +113,18 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     return tuple(_ext.load().qk_norm_rope_autograd(q, k, q_weight, k_weight, cos, sin, rot, positions, float(eps)))
 
 
+class _NotTwice(torch.autograd.Function):
+    """Gradients that cannot be differentiated again (under ``create_graph``): doing so raises."""
+
+    @staticmethod
+    def forward(ctx, *grads):
+        return grads
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("trying to differentiate twice a function whose backward is a kernel")
+
+
 class _QKNormAttention(torch.autograd.Function):
     """qk_norm_rope + flash attention on a packed QKV projection. One function, so that the backward
     writes dq, dk and dv into one packed gradient: attention's dq and dk land there, and the norm's
@@ -131,8 +142,15 @@ class _QKNormAttention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, do):
+        with torch.no_grad():
+            grads = _QKNormAttention._gradients(ctx, do)
+        if torch.is_grad_enabled():  # they depend on qkv and the weights, whether or not on a graph of `do`
+            grads = _NotTwice.apply(*(None if g is None else g.detach().requires_grad_(True) for g in grads))
+        return grads + (None,) * 8
+
+    @staticmethod
+    def _gradients(ctx, do):
         C = _ext.load()
         q, k, wq, wk, cos, sin, positions, qkv, yq, yk, o, lse, kv_len = ctx.saved_tensors
         dqkv = torch.empty_like(qkv)
@@ -143,7 +161,7 @@ class _QKNormAttention(torch.autograd.Function):
         _, _, dwq, dwk = C.qk_norm_rope_bwd(dq, dk, q, k, _f32(wq), _f32(wk), cos, sin, ctx.rot, positions,
                                             ctx.eps, need[0], need[1], acc[0], acc[1], dq, dk)
         dw = tuple(None if d is None else d.to(p.dtype) for d, p in zip((dwq, dwk), ctx.params))
-        return (dqkv,) + dw + (None,) * 8
+        return (dqkv,) + dw
 
 
 def qk_norm_attention_qkvpacked(qkv: torch.Tensor, q_weight: Optional[torch.Tensor] = None,

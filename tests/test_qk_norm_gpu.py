@@ -286,6 +286,30 @@ def test_packed_attention(rot):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("through", ["gradient", "input"])
+def test_second_derivatives_are_refused(packed, through):
+    """Gradients under ``create_graph`` have the right values; differentiating them raises, also when the
+    incoming gradient is no part of a graph (a penalty on the gradients would lose its own)."""
+    x = torch.randn(1, 30, 3, 2, 64, device="cuda").bfloat16().requires_grad_(True)
+    w = (torch.rand(64, device="cuda") + 0.5).requires_grad_(True)
+    dy = torch.randn(1, 30, 2, 64, device="cuda").bfloat16().requires_grad_(through == "gradient")
+
+    def run():
+        if packed:
+            return qk_norm_attention_qkvpacked(x, w, None)
+        return qk_norm_rope(x[:, :, 0], x[:, :, 1], w, None)[0]
+
+    want = torch.autograd.grad(run(), (x, w), dy.detach())
+    y = run()
+    got = torch.autograd.grad(y, (x, w), dy, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError, match="twice"):
+        (y.float().sum() + got[0].float().square().sum()).backward()
+    with pytest.raises(RuntimeError, match="twice"):
+        got[1].sum().backward()
+
+
 def test_captured_graph_replays():
     x = torch.randn(2, 65, 8, 64, device="cuda").bfloat16()
     g = torch.randn_like(x)
