@@ -10,6 +10,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+import torch.nn.functional as F
 
 from determined_clone_amd.ops import _ext, _grad
 from determined_clone_amd.ops.transformer import _attn_gpu_ok, _f32, _kv_len, reference_attention
@@ -26,8 +27,9 @@ def _reference_one(x, w, cos, sin, rot, positions, eps):
         y = y * w.to(wide)
     if rot:
         half = rot // 2
-        at = slice(0, x.shape[1]) if positions is None else positions.long()
-        c, s = cos[at].to(wide).unsqueeze(-2), sin[at].to(wide).unsqueeze(-2)
+        # (a lookup, not an index: those count negative positions from the end)
+        c, s = (t[:x.shape[1]] if positions is None else F.embedding(positions.long(), t) for t in (cos, sin))
+        c, s = c.to(wide).unsqueeze(-2), s.to(wide).unsqueeze(-2)
         a, b, rest = y[..., :half], y[..., half:rot], y[..., rot:]
         y = torch.cat([a * c - b * s, b * c + a * s, rest], dim=-1)
     return y.to(x.dtype)

@@ -71,3 +71,17 @@ def test_refusals():
         qk_norm_rope(q, k, wq, wk, cos, sin, positions=torch.full((5,), 5))
     with pytest.raises(ValueError, match="3, H, D"):
         qk_norm_attention_qkvpacked(torch.randn(2, 5, 2, 4, 8))
+
+
+@pytest.mark.parametrize("bad", [-1, -5, -6, 5])
+def test_positions_outside_the_tables_raise(bad):
+    q, k, wq, wk = _qk(dtype=torch.float32)
+    cos, sin = T.rope_tables(5, 8)
+    for dtype in (torch.int32, torch.int64):
+        pos = torch.tensor([0, 4, bad, 1, 2], dtype=dtype)
+        for p in (pos, pos.expand(2, 5)):
+            with pytest.raises(IndexError):
+                qk_norm_rope(q, k, wq, wk, cos, sin, positions=p)
+        with pytest.raises(IndexError):
+            qk_norm_attention_qkvpacked(torch.randn(1, 5, 3, 2, 8), wq, wk, cos, sin, positions=pos)
+    assert qk_norm_rope(q, k, wq, wk, positions=pos)[0].shape == q.shape  # nothing turns: not looked at
