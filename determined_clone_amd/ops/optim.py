@@ -528,7 +528,6 @@ def _list_kernel(grads: List[torch.Tensor], norm_type: float, max_norm: Optional
     kind = _NORM_KINDS.get(norm_type)
     if kind is None or not grads or not grads[0].is_cuda:
         return None
-    _grad.join()  # weight gradients still running on the side stream
     return _ext.load().grad_list_norm(grads, kind, max_norm)
 
 
@@ -539,6 +538,7 @@ def grad_norm(grads: Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Te
     one read of every tensor, sums in 64 bits, the same bits on every run."""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     norm_type = float(norm_type)
+    _grad.join()  # weight gradients still running on the side stream, whoever reads them next
     total = _list_kernel(grads, norm_type, None)
     return torch.nn.utils.get_total_norm(grads, norm_type).float() if total is None else total
 
@@ -558,6 +558,7 @@ def clip_grad_norm_(parameters: Any, max_norm: float, norm_type: float = 2.0,
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [p.grad for p in params if p.grad is not None]
     max_norm, norm_type = float(max_norm), float(norm_type)
+    _grad.join()  # weight gradients still running on the side stream, whoever reads them next
     # a norm that may be refused is looked at before anything is scaled
     total = _list_kernel(grads, norm_type, None if error_if_nonfinite else max_norm)
     if total is None:

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from determined_clone_amd import pytorch as det_pytorch
-from determined_clone_amd.ops import optim
+from determined_clone_amd.ops import _grad, optim
 
 
 def _params(empty=True):
@@ -51,3 +51,19 @@ def test_empty_single_and_refusals():
     assert torch.equal(p.grad.nan_to_num(7), kept.nan_to_num(7))
     with pytest.raises((TypeError, ValueError)):
         optim.clip_grad_norm_([p], "a lot")
+
+
+@pytest.mark.parametrize("norm_type", [2, 3])
+@pytest.mark.parametrize("refuse", [False, True])
+def test_side_stream_gradients_are_awaited_where_torch_clips(norm_type, refuse, monkeypatch):
+    """What the kernels do not take goes to torch, which must not read gradients still being written."""
+    calls = []
+    monkeypatch.setattr(_grad, "join", lambda: calls.append("join"))
+    for name in ("clip_grad_norm_", "get_total_norm"):
+        plain = getattr(torch.nn.utils, name)
+        monkeypatch.setattr(torch.nn.utils, name, lambda *a, f=plain, n=name, **k: (calls.append(n), f(*a, **k))[1])
+    optim.clip_grad_norm_(_params(), 0.5, norm_type, error_if_nonfinite=refuse)
+    assert calls[:2] == ["join", "clip_grad_norm_"]
+    calls.clear()
+    optim.grad_norm([p.grad for p in _params() if p.grad is not None], norm_type)
+    assert calls[:2] == ["join", "get_total_norm"]

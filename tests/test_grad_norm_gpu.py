@@ -182,6 +182,31 @@ def test_side_stream_gradients_land_first():
     torch.testing.assert_close(p.grad, torch.full_like(p, 1 / 2048.0), rtol=1e-5, atol=0)
 
 
+@pytest.mark.parametrize("kind", ["order 3", "CPU first"])
+def test_side_stream_gradients_land_before_torchs_clipping(kind):
+    p = torch.nn.Parameter(torch.zeros(1 << 20, device="cuda"))
+    p._dca_direct_grad = True
+    p.grad = torch.zeros_like(p)
+    side = _grad.side_stream_for(p)
+    if side is None:
+        pytest.skip("side stream is off")
+    a = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    _grad.fork(side, (a,))
+    with torch.cuda.stream(side):
+        for _ in range(10):
+            a = a @ a * 1e-2
+        p.grad.add_(1.0)
+    params, order = [p], 3.0
+    if kind == "CPU first":
+        params, order = [torch.nn.Parameter(torch.zeros(4)), p], 2.0
+        params[0].grad = torch.zeros(4)
+    want = float(1 << 20) ** (1 / order)
+    # torch's norm: its own order of 2^20 fp32 additions of ones and a root; all of them exact but the root
+    assert abs(float(optim.clip_grad_norm_(params, 1.0, order)) - want) <= 1e-5 * want
+    torch.testing.assert_close(p.grad, torch.full_like(p, 1 / want), rtol=2e-5, atol=0)
+
+
 def test_captured_graph_replays():
     grads = _grads([3001, 70000, 5] * 80, [torch.bfloat16, torch.float32])
     ps = _params(grads)
