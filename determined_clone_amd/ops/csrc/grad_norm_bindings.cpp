@@ -12,12 +12,15 @@ using torch::Tensor;
 
 hipStream_t stream() { return at::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream(); }
 
+// Tensor subclasses, which may have no memory of their own.
+bool wrapped(const Tensor& g) { return g.unsafeGetTensorImpl()->key_set().has(c10::DispatchKey::Python); }
+
 // Whether two of the tensors share memory (each taken from its first to its last element).
 bool overlaps(const std::vector<Tensor>& grads) {
   std::vector<std::pair<const char*, const char*>> spans;
   spans.reserve(grads.size());
   for (const Tensor& g : grads) {
-    if (!g.defined() || g.layout() != at::kStrided || !g.numel()) continue;
+    if (!g.defined() || g.is_nested() || g.layout() != at::kStrided || wrapped(g) || !g.numel()) continue;
     int64_t last = 0;
     for (int64_t d = 0; d < g.dim(); ++d) last += (g.size(d) - 1) * g.stride(d);
     const char* p = static_cast<const char*>(g.data_ptr());
@@ -34,9 +37,9 @@ bool overlaps(const std::vector<Tensor>& grads) {
 bool describe(const std::vector<Tensor>& grads, bool write, std::vector<dca::GradTensor>& out) {
   out.reserve(grads.size());
   for (const Tensor& g : grads) {
-    if (!g.defined() || g.layout() != at::kStrided || !g.is_cuda() || g.device() != grads[0].device() ||
-        g.is_conj() || g.is_neg() || g.unsafeGetTensorImpl()->key_set().has(c10::DispatchKey::Python))
-      return false;  // (the last: tensor subclasses, which may have no memory of their own)
+    if (!g.defined() || g.is_nested() || g.layout() != at::kStrided || !g.is_cuda() || g.device() != grads[0].device() ||
+        g.is_conj() || g.is_neg() || wrapped(g))
+      return false;
     dca::TDtype dt;
     switch (g.scalar_type()) {
       case at::kBFloat16: dt = dca::TDtype::kBF16; break;

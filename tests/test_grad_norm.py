@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from determined_clone_amd import pytorch as det_pytorch
-from determined_clone_amd.ops import _grad, optim
+from determined_clone_amd.ops import _ext, _grad, optim
 
 
 def _params(empty=True):
@@ -67,3 +67,15 @@ def test_side_stream_gradients_are_awaited_where_torch_clips(norm_type, refuse, 
     calls.clear()
     optim.grad_norm([p.grad for p in _params() if p.grad is not None], norm_type)
     assert calls[:2] == ["join", "get_total_norm"]
+
+
+def test_overlap_is_asked_of_memory_only():
+    """Wrapper subclasses (sharded tensors) and nested tensors have no address to compare."""
+    from torch.testing._internal.two_tensor import TwoTensor
+
+    overlaps = _ext.load().grad_list_overlaps
+    x = torch.randn(100)
+    wrapped = [TwoTensor(torch.randn(3), torch.randn(3)) for _ in range(2)]
+    nested = [torch.nested.nested_tensor([torch.randn(2), torch.randn(3)]) for _ in range(2)]
+    assert not overlaps(wrapped) and not overlaps(nested) and not overlaps(wrapped + nested + [x[:50], x[50:]])
+    assert overlaps(wrapped + nested + [x[:51], x[50:]])
