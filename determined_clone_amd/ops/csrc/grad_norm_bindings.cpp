@@ -53,6 +53,13 @@ bool describe(const std::vector<Tensor>& grads, bool write, std::vector<dca::Gra
   return !write || !overlaps(grads);
 }
 
+// Scales the tensors; autograd hears of it, as of any change in place.
+void clip(const std::vector<Tensor>& grads, const std::vector<dca::GradTensor>& t, const Tensor& norm, double max_norm) {
+  dca::grad_clip(t, norm.data_ptr<float>(), static_cast<float>(max_norm), stream());
+  for (const Tensor& g : grads)
+    if (!g.is_inference()) g.unsafeGetTensorImpl()->bump_version();
+}
+
 // kind: 0 L2, 1 L1, 2 max. -> the fp32 norm, or None where the kernels do not apply. With max_norm
 // the tensors are also scaled by min(1, max_norm / (norm + 1e-6)).
 c10::optional<Tensor> grad_list_norm(const std::vector<Tensor>& grads, int64_t kind, c10::optional<double> max_norm) {
@@ -63,7 +70,7 @@ c10::optional<Tensor> grad_list_norm(const std::vector<Tensor>& grads, int64_t k
   Tensor ws = torch::empty({dca::grad_norm_workspace(t)}, grads[0].options().dtype(at::kDouble));
   Tensor norm = torch::empty({}, grads[0].options().dtype(at::kFloat));
   dca::grad_norm(t, static_cast<dca::NormKind>(kind), ws.data_ptr<double>(), norm.data_ptr<float>(), stream());
-  if (max_norm.has_value()) dca::grad_clip(t, norm.data_ptr<float>(), static_cast<float>(*max_norm), stream());
+  if (max_norm.has_value()) clip(grads, t, norm, *max_norm);
   return norm;
 }
 
@@ -74,7 +81,7 @@ c10::optional<Tensor> grad_list_clip(const std::vector<Tensor>& grads, const Ten
   TORCH_CHECK(norm.scalar_type() == at::kFloat && norm.numel() == 1 && norm.device() == grads[0].device(),
               "grad_list_clip: the norm must be one fp32 value on the gradients' device");
   const c10::DeviceGuard g(grads[0].device());
-  dca::grad_clip(t, norm.data_ptr<float>(), static_cast<float>(max_norm), stream());
+  clip(grads, t, norm, max_norm);
   return norm;
 }
 }  // namespace

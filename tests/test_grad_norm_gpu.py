@@ -182,6 +182,24 @@ def test_side_stream_gradients_land_first():
     torch.testing.assert_close(p.grad, torch.full_like(p, 1 / 2048.0), rtol=1e-5, atol=0)
 
 
+@pytest.mark.parametrize("refuse", [False, True])
+def test_autograd_hears_of_the_scaling(refuse):
+    """A gradient that another graph has saved: its backward raises after clipping rather than use it."""
+    p, = _params(_grads([300], [torch.float32]))
+    x = torch.randn(300, device="cuda", requires_grad=True)
+    y = x * p.grad
+    optim.grad_norm([p.grad])
+    torch.autograd.grad(y.sum(), x, retain_graph=True)  # a norm changes nothing
+    optim.clip_grad_norm_([p], 1e-3, error_if_nonfinite=refuse)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():
+        q = torch.zeros(3, device="cuda")
+        q.grad = torch.full((3,), 2.0, device="cuda")
+        optim.clip_grad_norm_([q], 1.0, error_if_nonfinite=refuse)
+        assert float(q.grad.square().sum()) < 1.001
+
+
 @pytest.mark.parametrize("kind", ["order 3", "CPU first"])
 def test_side_stream_gradients_land_before_torchs_clipping(kind):
     p = torch.nn.Parameter(torch.zeros(1 << 20, device="cuda"))
