@@ -305,10 +305,11 @@ constexpr int kDirectWaves = 4;
 constexpr int kDirectUnroll = 8;
 template <typename T, bool kAligned>
 __global__ __launch_bounds__(kDirectWaves * 64) void embed_grad_direct_kernel(
-    EmbedIds ids, const void* __restrict__ dy, void* __restrict__ out, int E, float scale, bool accumulate) {
+    int64_t block0, EmbedIds ids, const void* __restrict__ dy, void* __restrict__ out, int E, float scale,
+    bool accumulate) {
   constexpr int V = kFull<T>;
   const int lane = threadIdx.x & 63;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kDirectWaves + (threadIdx.x >> 6);
+  const int64_t row = (block0 + blockIdx.x) * kDirectWaves + (threadIdx.x >> 6);
   if (row >= ids.rows) return;
   const int c = (blockIdx.y * 64 + lane) * V;
   const bool ok = c < E;
@@ -352,17 +353,17 @@ __global__ __launch_bounds__(kDirectWaves * 64) void embed_grad_direct_kernel(
 // range (its "head"), 1 of one that began here and goes on (its "tail").
 constexpr int kGradUnroll = 8;
 template <typename T, bool kAligned, bool kAdd>
-__global__ __launch_bounds__(256) void embed_grad_kernel(const uint64_t* __restrict__ sorted,
+__global__ __launch_bounds__(256) void embed_grad_kernel(int64_t block0, const uint64_t* __restrict__ sorted,
                                                          const void* __restrict__ dy, void* out,
                                                          float* __restrict__ partial, int64_t n, int E, int K,
                                                          float scale) {
   constexpr int V = kFull<T>;
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
   const bool ok = c < E;
-  const int64_t lo = static_cast<int64_t>(blockIdx.x) * K;
+  const int64_t x = block0 + blockIdx.x, lo = x * K;
   const int cnt = static_cast<int>(n - lo < K ? n - lo : K);
   const int64_t ps = partial_stride(E);
-  float* head = partial + static_cast<int64_t>(blockIdx.x) * 2 * ps;
+  float* head = partial + x * 2 * ps;
   const int lane = threadIdx.x & 63;
   const uint64_t entry = sorted[lo + (lane < cnt ? lane : cnt - 1)];
   const int before = lo > 0 ? row_of(sorted[lo - 1]) : -1;
@@ -445,12 +446,13 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const uint64_t* __restr
 // the following ranges to its tail. 4 waves take every fourth range, 256 columns a workgroup.
 constexpr int kJoinWaves = 4;
 template <typename T>
-__global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(const uint64_t* __restrict__ sorted,
+__global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(int64_t block0,
+                                                                     const uint64_t* __restrict__ sorted,
                                                                      const float* __restrict__ partial,
                                                                      void* __restrict__ out, int64_t n, int E,
                                                                      int K, float scale, bool accumulate) {
   __shared__ float4 red[kJoinWaves][64];
-  const int64_t lo = static_cast<int64_t>(blockIdx.x) * K, hi = lo + K;
+  const int64_t x = block0 + blockIdx.x, lo = x * K, hi = lo + K;
   if (hi >= n) return;
   const int row = row_of(sorted[hi - 1]), next = row_of(sorted[hi]), first = row_of(sorted[lo]);
   const int before = row_of(sorted[lo > 0 ? lo - 1 : 0]);
@@ -458,7 +460,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(const uint6
   if (lo > 0 && first == row && before == row) return;  // began earlier
   // the last range that begins with the token (they follow each other): 64 ranges a step, since a step
   // costs a trip to memory, 64 times as far apart while all have it, and back
-  const int64_t x = blockIdx.x, nb = (n + K - 1) / K;
+  const int64_t nb = (n + K - 1) / K;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int64_t last = x;
   for (int64_t apart = 1; apart;) {
@@ -500,12 +502,13 @@ __global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(const uint6
 // in a fixed order.
 constexpr int kSumUnroll = 8;
 template <typename T, bool kAligned>
-__global__ __launch_bounds__(1024) void batch_sum_kernel(const void* __restrict__ dy, void* __restrict__ out,
+__global__ __launch_bounds__(1024) void batch_sum_kernel(int64_t block0, const void* __restrict__ dy,
+                                                         void* __restrict__ out,
                                                          int64_t B, int64_t N, bool accumulate) {
   constexpr int V = kFull<T>;
   extern __shared__ float red[];  // [waves][64][V]
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  const int64_t c = (static_cast<int64_t>(blockIdx.x) * 64 + lane) * V;
+  const int64_t c = ((block0 + blockIdx.x) * 64 + lane) * V;
   float a[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) a[k] = 0.f;
@@ -566,6 +569,15 @@ int grad_range(int64_t n) { return n >= 16384 ? 32 : (n >= 4096 ? 16 : 8); }
 // 256 ids 28 against 23). All ids the same is the sort's better case: 256 of them 31 against 13 us.
 bool direct(int64_t n, int64_t rows) { return n <= 128 || (n <= 256 && rows <= 4096); }
 
+// f(first workgroup, workgroups) for the launches that `blocks` workgroups take: HIP refuses 2^32
+// threads and more in one.
+constexpr int64_t kMaxBlocks = 1 << 21;
+template <typename F>
+void for_blocks(int64_t blocks, F&& f) {
+  for (int64_t b = 0; b < blocks; b += kMaxBlocks)
+    f(b, static_cast<unsigned>(blocks - b < kMaxBlocks ? blocks - b : kMaxBlocks));
+}
+
 int64_t partial_floats(int64_t n, int E) {
   const int64_t K = grad_range(n);
   return (n + K - 1) / K * 2 * ((E + 3) & ~3);
@@ -580,10 +592,11 @@ void embed_fwd(TDtype dt, bool aligned, const EmbedIds& ids, const void* table, 
     constexpr int V = kFull<T>;
     constexpr bool A = decltype(a)::value;
     const int64_t nv = (E + V - 1) / V;
-    // one pass of the workgroup's unrolled loop, as long as that leaves 1024 workgroups
+    // one pass of the workgroup's unrolled loop, as long as that leaves 1024 workgroups, and rows enough
+    // for one launch
     int64_t r = kFwdBlock * kFwdUnroll / nv;
     if (r > ids.n / 1024) r = ids.n / 1024;
-    if (r < 1) r = 1;
+    if (r <= ids.n / kMaxBlocks) r = ids.n / kMaxBlocks + 1;
     auto* kernel = ids.n * E * kElem<T> >= kStreamBytes ? embed_fwd_kernel<T, A, true> : embed_fwd_kernel<T, A, false>;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((ids.n + r - 1) / r)), dim3(kFwdBlock), 0, st, ids, table,
                        stride, pos, scale, out, E, static_cast<int>(r));
@@ -623,10 +636,11 @@ void embed_grad(TDtype dt, bool aligned, const EmbedIds& ids, const void* dy, vo
       using T = decltype(t);
       constexpr int V = kFull<T>;
       constexpr bool A = decltype(a)::value;
-      hipLaunchKernelGGL((embed_grad_direct_kernel<T, A>),
-                         dim3(static_cast<unsigned>((ids.rows + kDirectWaves - 1) / kDirectWaves),
-                              static_cast<unsigned>((E + 64 * V - 1) / (64 * V))),
-                         dim3(kDirectWaves * 64), 0, st, ids, dy, out, E, scale, accumulate);
+      for_blocks((ids.rows + kDirectWaves - 1) / kDirectWaves, [&](int64_t first, unsigned blocks) {
+        hipLaunchKernelGGL((embed_grad_direct_kernel<T, A>),
+                           dim3(blocks, static_cast<unsigned>((E + 64 * V - 1) / (64 * V))), dim3(kDirectWaves * 64),
+                           0, st, first, ids, dy, out, E, scale, accumulate);
+      });
     });
     return;
   }
@@ -636,23 +650,23 @@ void embed_grad(TDtype dt, bool aligned, const EmbedIds& ids, const void* dy, vo
   if (ids.ids.is32) place<int32_t>(ids, sorted, out, clear, st);
   else place<int64_t>(ids, sorted, out, clear, st);
   const int K = grad_range(n);
-  const unsigned nb = static_cast<unsigned>((n + K - 1) / K);
+  const int64_t nb = (n + K - 1) / K;
   dispatch_ta(dt, aligned, [&](auto t, auto a) {
     using T = decltype(t);
     constexpr int V = kFull<T>;
     constexpr bool A = decltype(a)::value;
     const int nv = (E + V - 1) / V;
     const int threads = nv >= 256 ? 256 : (nv + 63) / 64 * 64;
-    const dim3 grid(nb, static_cast<unsigned>((nv + threads - 1) / threads));
-    if (accumulate)
-      hipLaunchKernelGGL((embed_grad_kernel<T, A, true>), grid, dim3(threads), 0, st, sorted, dy, out, partial,
-                         n, E, K, scale);
-    else
-      hipLaunchKernelGGL((embed_grad_kernel<T, A, false>), grid, dim3(threads), 0, st, sorted, dy, out, partial,
-                         n, E, K, scale);
-    if (nb > 1)
-      hipLaunchKernelGGL(embed_join_kernel<T>, dim3(nb, static_cast<unsigned>((E + 255) / 256)),
-                         dim3(kJoinWaves * 64), 0, st, sorted, partial, out, n, E, K, scale, accumulate);
+    auto* kernel = accumulate ? embed_grad_kernel<T, A, true> : embed_grad_kernel<T, A, false>;
+    for_blocks(nb, [&](int64_t first, unsigned blocks) {
+      hipLaunchKernelGGL(kernel, dim3(blocks, static_cast<unsigned>((nv + threads - 1) / threads)), dim3(threads), 0,
+                         st, first, sorted, dy, out, partial, n, E, K, scale);
+    });
+    if (nb == 1) return;
+    for_blocks(nb, [&](int64_t first, unsigned blocks) {
+      hipLaunchKernelGGL(embed_join_kernel<T>, dim3(blocks, static_cast<unsigned>((E + 255) / 256)),
+                         dim3(kJoinWaves * 64), 0, st, first, sorted, partial, out, n, E, K, scale, accumulate);
+    });
   });
 }
 
@@ -666,9 +680,11 @@ void batch_sum(TDtype dt, bool aligned, const void* dy, void* out, int64_t B, in
     const int64_t tiles = (N + 64 * V - 1) / (64 * V);
     int waves = 1;  // split the batch where the columns alone do not fill the chip
     while (waves < 16 && waves * 2 <= B && tiles * waves < 4096) waves *= 2;
-    hipLaunchKernelGGL((batch_sum_kernel<T, A>), dim3(static_cast<unsigned>(tiles)), dim3(waves * 64),
-                       waves > 1 ? static_cast<size_t>(waves) * 64 * V * sizeof(float) : 0, st, dy, out, B, N,
-                       accumulate);
+    for_blocks(tiles, [&](int64_t first, unsigned blocks) {
+      hipLaunchKernelGGL((batch_sum_kernel<T, A>), dim3(blocks), dim3(waves * 64),
+                         waves > 1 ? static_cast<size_t>(waves) * 64 * V * sizeof(float) : 0, st, first, dy, out, B, N,
+                         accumulate);
+    });
   });
 }
 }  // namespace dca

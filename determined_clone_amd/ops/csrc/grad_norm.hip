@@ -197,7 +197,9 @@ Walk walk_of(const std::vector<GradTensor>& t) {
   }
   int64_t c = 2048;  // small lists: workgroups for every CU
   while (c < 32768 && total / c > 2048) c *= 2;
-  return {c, c < 8192 ? c : 8192, bytes > 256 << 20};
+  int64_t clip = c < 8192 ? c : 8192;
+  while (total / clip > 1 << 22) clip *= 2;  // HIP refuses launches of 2^32 threads
+  return {c, clip, bytes > 256 << 20};
 }
 
 // f(table, workgroups) for every launch of the list

@@ -223,6 +223,34 @@ def test_far_offsets():
     assert torch.equal(dw[v - 2], dy[0, 2]) and torch.equal(dw[0], dy[0, 1])
 
 
+@pytest.mark.parametrize("n", [100, 1000])
+@pytest.mark.parametrize("add", [False, True])
+def test_a_table_of_many_rows(n, add):
+    """More rows than one launch has waves for."""
+    v, e = 2 ** 26 + 11, 8
+    g = torch.Generator(device="cuda").manual_seed(n)
+    idx = torch.randint(0, v, (1, n), generator=g, device="cuda")
+    idx[0, :5] = torch.tensor([v - 1, 0, 2 ** 25, v - 1, v], device="cuda")  # the last one has no row
+    dy = torch.randn(1, n, e, generator=g, device="cuda").bfloat16()
+    acc = torch.zeros(v, e, device="cuda", dtype=torch.bfloat16) if add else None
+    dw = _ext.load().embed_grad(dy, idx, v, acc=acc)
+    rows, where = idx[idx < v].unique(return_inverse=True)
+    _check_grad(dw[rows], dy[:, idx[0] < v], where[None], len(rows))
+    assert int(dw.any(1).sum()) == int(dw[rows].any(1).sum())
+
+
+def test_many_ids():
+    """More workgroups than one launch takes (2^29 ids of a long axis)."""
+    n, v = 2 ** 29 + 100, 1000
+    g = torch.Generator(device="cuda").manual_seed(0)
+    idx = torch.randint(0, v, (n,), generator=g, device="cuda", dtype=torch.int32)
+    idx[-50:] = 7
+    dw = _ext.load().embed_grad(torch.ones(n, 1, device="cuda", dtype=torch.bfloat16), idx, v)
+    counts = torch.bincount(idx, minlength=v)
+    assert int(counts.max()) < 2 ** 24  # so that the fp32 sums of ones are exact
+    assert torch.equal(dw[:, 0], counts.float().bfloat16())
+
+
 def test_captured_graph_replays():
     idx, w, p, dy = _inputs(4, 2500, 400, 64, torch.bfloat16, seed=8, p=2500)
     C = _ext.load()
