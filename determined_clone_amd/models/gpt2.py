@@ -94,7 +94,13 @@ class FusedLayerNorm(nn.Module):
 
 
 class TokenEmbedding(nn.Embedding):
-    """Token table; ``forward(idx, pos_weight)`` adds the rows of a learned-position table."""
+    """Token table; ``forward(idx, pos_weight)`` adds the rows of a learned-position table. The
+    options of ``nn.Embedding`` that change a lookup or its gradient are refused."""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, **kw) -> None:
+        super().__init__(num_embeddings, embedding_dim, **kw)
+        if self.padding_idx is not None or self.max_norm is not None or self.scale_grad_by_freq or self.sparse:
+            raise ValueError("TokenEmbedding: padding_idx, max_norm, scale_grad_by_freq and sparse are not supported")
 
     def forward(self, idx: torch.Tensor, pos_weight: Optional[torch.Tensor] = None) -> torch.Tensor:
         return embedding(idx, self.weight, pos_weight)

@@ -69,6 +69,17 @@ def test_without_qk_norm_nothing_is_added():
     assert m.blocks[0].attn.q_norm.weight.dtype == torch.float32  # kept like LayerNorm's
 
 
+def test_token_embedding_refuses_what_its_lookup_does_not_do():
+    for kw in (dict(padding_idx=0), dict(max_norm=1.0), dict(scale_grad_by_freq=True), dict(sparse=True)):
+        with pytest.raises(ValueError, match="not supported"):
+            gpt2.TokenEmbedding(4, 2, **kw)
+        with pytest.raises(ValueError, match="not supported"):
+            gpt2.TokenEmbedding.from_pretrained(torch.ones(4, 2), **kw)
+    t = gpt2.TokenEmbedding(4, 2, device="cpu", dtype=torch.float64)
+    assert t(torch.tensor([3])).dtype == torch.float64
+    assert torch.equal(gpt2.TokenEmbedding.from_pretrained(torch.ones(4, 2))(torch.tensor([1])), torch.ones(1, 2))
+
+
 def _tp_parity(rank, world, d, pos):
     torch.manual_seed(0)
     cfg = gpt2.config_for("tiny", n_layer=2, n_head=4, d_model=256, vocab_size=500, max_seq_len=32, pos_emb=pos,
