@@ -12,6 +12,7 @@ the rows of tokens that occur are touched, added in place; otherwise a dense gra
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.nn.functional as F
 
 from determined_clone_amd.ops import _ext
@@ -37,6 +38,17 @@ def reference_embedding(idx, weight, pos_weight=None, positions=None, scale=1.0,
     return out.to(weight.dtype)
 
 
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def _kernel_takes(weight: torch.Tensor, pos_weight: Optional[torch.Tensor] = None) -> bool:
+    """Whether the tables (of one dtype and device) are plain GPU tensors outside of function transforms
+    (vmap, jvp, grad, ...) and forward-mode differentiation, which the kernels' node does not know."""
+    return (weight.is_cuda and weight.dtype in _DTYPES and type(weight) in _PLAIN
+            and (pos_weight is None or type(pos_weight) in _PLAIN)
+            and forward_ad._current_level < 0 and torch._C._functorch.peek_interpreter_stack() is None)
+
+
 def _check_index(t: torch.Tensor, what: str) -> None:
     if t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"embedding: {what} must be int32 or int64, got {t.dtype}")
@@ -55,8 +67,12 @@ def embedding(idx: torch.Tensor, weight: torch.Tensor, pos_weight: Optional[torc
     ``vocab_start`` makes ``weight`` a shard of a larger vocabulary, rows ``vocab_start`` and up: ids
     outside it look up zeros and have no gradient (sum the shards' outputs with an all-reduce).
     Without it every id has to lie in [0, V), and every position in [0, P): the CPU path raises
-    ``IndexError`` for others, the GPU path, which does not wait for the values, returns NaN rows
-    for them and gives them no gradient in the table that they miss."""
+    ``IndexError`` for others, the GPU kernels, which do not wait for the values, return NaN rows
+    for them and give them no gradient in the table that they miss.
+
+    float64 tables, tensor subclasses, function transforms (``torch.func``) and forward-mode
+    differentiation run as plain PyTorch on the GPU too, where a mistaken id ends the program.
+    Second derivatives through the kernels raise."""
     _check_index(idx, "idx")
     if weight.dim() != 2 or not weight.is_floating_point():
         raise ValueError("embedding: weight must be a floating-point [V, E] table")
@@ -82,7 +98,7 @@ def embedding(idx: torch.Tensor, weight: torch.Tensor, pos_weight: Optional[torc
             raise ValueError("embedding: a single id needs its position")
         elif idx.shape[-1] > pos_weight.shape[0]:
             raise ValueError(f"embedding: {idx.shape[-1]} tokens, {pos_weight.shape[0]} positions")
-    if not weight.is_cuda or weight.dtype not in _DTYPES:  # float64 tables: plain PyTorch
+    if not _kernel_takes(weight, pos_weight):
         return reference_embedding(idx, weight, pos_weight, positions, scale, vocab_start)
     return _ext.load().embedding(idx, weight, pos_weight, positions, float(scale), vocab_start or 0,
                                  vocab_start is not None)

@@ -82,3 +82,33 @@ def test_refusals():
         embedding(idx + 5, w)
     with pytest.raises(IndexError):
         embedding(idx, w, w, positions=idx - 1)
+
+
+def test_what_the_kernels_are_asked_for(monkeypatch):
+    """Plain tables in three types; not float64, not subclasses, nothing under transforms or forward mode."""
+    from determined_clone_amd.ops import embedding as E
+
+    class Table(torch.Tensor):
+        pass
+
+    asked = []
+
+    def ask(*tables):
+        with monkeypatch.context() as m:
+            m.setattr(torch.Tensor, "is_cuda", True)  # as on a GPU
+            asked.append(E._kernel_takes(*tables))
+        return tables[0]
+
+    w = torch.randn(5, 4)
+    assert not E._kernel_takes(w)
+    for t in (w, w.half(), w.bfloat16(), torch.nn.Parameter(w)):
+        ask(t), ask(t, t)
+    assert asked == [True] * 8
+    asked.clear()
+    ask(w.double()), ask(w.as_subclass(Table)), ask(w, w.as_subclass(Table))
+    torch.vmap(lambda i: ask(w) + i)(w)
+    torch.func.jvp(ask, (w,), (w,))
+    torch.func.grad(lambda a: ask(a).sum())(w)
+    with torch.autograd.forward_ad.dual_level():
+        ask(w)
+    assert asked == [False] * 7

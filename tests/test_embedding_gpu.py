@@ -292,6 +292,27 @@ def test_float64_tables_take_plain_torch():
     torch.testing.assert_close(embedding(idx, w.double(), p.double(), scale=2.0), 2 * w.double()[idx] + p.double()[:6])
 
 
+def test_transforms_and_forward_mode_take_plain_torch():
+    idx, w, p, dy = _inputs(3, 6, 30, 16, torch.float32, p=8)
+    t = torch.randn_like(w)
+    want = w[idx] * 2.0 + p[:6]
+    run = lambda i, a: embedding(i, a, p, scale=2.0)  # noqa: E731
+    assert torch.equal(torch.vmap(run, (0, None))(idx, w), want)
+    for out, tangent in (torch.func.jvp(lambda a: run(idx, a), (w,), (t,)), _dual(lambda a: run(idx, a), w, t)):
+        assert torch.equal(out, want) and torch.equal(tangent, t[idx] * 2.0)
+    torch.testing.assert_close(torch.func.grad(lambda a: (run(idx, a) * dy).sum())(w),
+                               _ext.load().embed_grad(dy, idx, 30, 2.0), rtol=1e-5, atol=1e-5)
+    shard = torch.vmap(lambda i: embedding(i, w[:10], vocab_start=0))(idx)
+    assert torch.equal(shard, embedding(idx, w[:10], vocab_start=0))
+
+
+def _dual(f, x, t):
+    import torch.autograd.forward_ad as fw
+
+    with fw.dual_level():
+        return tuple(fw.unpack_dual(f(fw.make_dual(x, t))))
+
+
 def test_refusals():
     w = torch.randn(5, 4, device="cuda")
     idx = torch.zeros(2, 3, dtype=torch.long, device="cuda")
