@@ -22,13 +22,17 @@ _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 def reference_embedding(idx, weight, pos_weight=None, positions=None, scale=1.0, vocab_start=None):
     """The same operator in plain PyTorch (fp32 or wider arithmetic, rounded once)."""
-    local = idx.long() - (vocab_start or 0)
-    wide = torch.promote_types(weight.dtype, torch.float32)
+    local = idx.long() - vocab_start if vocab_start else idx.long()
+    # without a product the one sum is rounded once in the tables' own type
+    wide = weight.dtype if scale == 1 else torch.promote_types(weight.dtype, torch.float32)
     if vocab_start is None:
-        out = F.embedding(local, weight).to(wide) * scale
+        out = F.embedding(local, weight)
     else:
         outside = (local < 0) | (local >= weight.shape[0])
-        out = F.embedding(local.masked_fill(outside, 0), weight).to(wide) * scale
+        out = F.embedding(local.masked_fill(outside, 0), weight)
+    if scale != 1:
+        out = out.to(wide) * scale
+    if vocab_start is not None:
         out = out.masked_fill(outside.unsqueeze(-1), 0)
     if pos_weight is not None:
         if positions is None:

@@ -112,3 +112,32 @@ def test_what_the_kernels_are_asked_for(monkeypatch):
     with torch.autograd.forward_ad.dual_level():
         ask(w)
     assert asked == [False] * 7
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_plain_lookup_on_the_cpu_is_one_pass(dtype):
+    """No copies to fp32 and no product with 1 around the lookup (and the addition of positions)."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Count(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.passes = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            if isinstance(out, torch.Tensor) and out.is_floating_point() and not func.is_view:
+                self.passes.append(func.overloadpacket.__name__)
+            return out
+
+    g = torch.Generator().manual_seed(3)
+    w, p = torch.randn(30, 16, generator=g).to(dtype), torch.randn(9, 16, generator=g).to(dtype)
+    idx = torch.randint(0, 30, (4, 9), generator=g)
+    for call, want, ops in ((lambda: embedding(idx, w), w[idx], ["embedding"]),
+                            (lambda: embedding(idx, w, p), (w[idx].double() + p.double()).to(dtype), ["embedding", "add"]),
+                            (lambda: embedding(idx, w[:20], vocab_start=0), w[idx] * (idx < 20)[..., None],
+                             ["embedding", "masked_fill"])):
+        with Count() as count:
+            out = call()
+        assert count.passes == ops
+        assert torch.equal(out, want)
