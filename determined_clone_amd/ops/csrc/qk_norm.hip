@@ -102,9 +102,13 @@ __device__ __forceinline__ void load_angles(const QkShape& s, const float* __res
   }
 }
 
-// 1 / sqrt(mean + eps): v_rsq_f32 is within 1 ulp, below the rounding of the sum that it takes.
+// 1 / sqrt(mean + eps): v_rsq_f32 is within 1 ulp, below the rounding of the sum that it takes. It
+// takes subnormal numbers (tiny rows without an eps) for 0: those are raised by 2^64 before it.
 __device__ __forceinline__ float rms_inv(float sum, float inv_d, float eps) {
-  return __builtin_amdgcn_rsqf(sum * inv_d + eps);
+  const float m = sum * inv_d + eps;
+  const bool tiny = m < 0x1p-126f;
+  const float r = __builtin_amdgcn_rsqf(tiny ? m * 0x1p64f : m);
+  return tiny ? r * 0x1p32f : r;
 }
 
 __device__ __forceinline__ int64_t head_offset(const HeadView& v, int64_t b, int64_t t, int h) {

@@ -172,6 +172,24 @@ def test_zero_rows_and_large_values():
     assert y[0, 3, 0, 5] == 8.0 and y[0, 3].float().abs().sum() == 8.0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [64, 33])
+def test_tiny_rows_without_an_eps(dtype, d):
+    """Mean squares below 2^-126. A square there is off by up to 2^-150, here 2^-23 of the mean square at
+    most, its root by half of that: one of the steps that the bounds count."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = [(torch.rand(2, 9, 2, d, generator=g, device="cuda") * 0.2 + 0.9).mul(0.9e-19).to(dtype).requires_grad_(True)
+         for _ in range(2)]
+    w = [(torch.rand(d, generator=g, device="cuda") + 0.5).requires_grad_(True) for _ in range(2)]
+    dy = [torch.randn(2, 9, 2, d, generator=g, device="cuda").to(dtype) for _ in range(2)]
+    assert x[0].double().square().mean(-1).max() < 2.0 ** -126 and x[0].double().square().mean(-1).min() > 2.0 ** -127
+    y = qk_norm_rope(*x, *w, eps=0.0)
+    grads = torch.autograd.grad(y, x + w, dy)
+    for i in range(2):
+        _check(x[i], w[i], dy[i], None, None, 0, None, 0.0, y[i].detach(), grads[i], grads[2 + i])
+    assert torch.isnan(qk_norm_rope(torch.zeros_like(x[0]), x[1], eps=0.0)[0]).all()  # 0 / 0
+
+
 def test_strides():
     g = torch.Generator(device="cuda").manual_seed(3)
     x = torch.randn(2, 4, 30, 64, generator=g, device="cuda").bfloat16()  # [B, H, S, D]
