@@ -111,10 +111,6 @@ __device__ __forceinline__ float rms_inv(float sum, float inv_d, float eps) {
   return tiny ? r * 0x1p32f : r;
 }
 
-__device__ __forceinline__ int64_t head_offset(const HeadView& v, int64_t b, int64_t t, int h) {
-  return b * v.sb + t * v.ss + h * v.sh;
-}
-
 // U groups of heads at once: their loads leave together, before the first is used.
 template <typename T, int V, int L, int NV, int U>
 __global__ __launch_bounds__(kQkBlock) void qk_fwd_kernel(QkShape s, HeadView xq, HeadView xk, HeadView yq,
