@@ -106,6 +106,16 @@ class TokenEmbedding(nn.Embedding):
         return embedding(idx, self.weight, pos_weight)
 
 
+def _embed(wte: nn.Module, wpe: Optional[nn.Embedding], idx: torch.Tensor) -> torch.Tensor:
+    """Token rows, plus learned positions where there are any: in one pass, unless another module has
+    taken the token table's place (a larger vocabulary, an adapter)."""
+    if wpe is None:
+        return wte(idx)
+    if isinstance(wte, TokenEmbedding):
+        return wte(idx, wpe.weight)
+    return wte(idx) + wpe.weight[:idx.shape[1]].unsqueeze(0)
+
+
 class HeadNorm(nn.Module):
     """Weight of the RMS norm of the query or key heads, applied by the attention op."""
 
@@ -239,7 +249,7 @@ class GPT(nn.Module):
         return float(dense + attn)
 
     def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None):
-        x = self.wte(idx, None if self.wpe is None else self.wpe.weight)
+        x = _embed(self.wte, self.wpe, idx)
         rope = (self.rope_cos, self.rope_sin) if self.cfg.pos_emb == "rotary" else None
         resid, delta = x, None
         for blk in self.blocks:
@@ -278,7 +288,7 @@ class EmbeddingPipe(nn.Module):
         _init_like_gpt(self, cfg)
 
     def forward(self, idx: torch.Tensor) -> torch.Tensor:
-        return self.wte(idx, None if self.wpe is None else self.wpe.weight)
+        return _embed(self.wte, self.wpe, idx)
 
 
 class BlockPipe(Block):

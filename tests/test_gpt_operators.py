@@ -80,6 +80,21 @@ def test_token_embedding_refuses_what_its_lookup_does_not_do():
     assert torch.equal(gpt2.TokenEmbedding.from_pretrained(torch.ones(4, 2))(torch.tensor([1])), torch.ones(1, 2))
 
 
+@pytest.mark.parametrize("pos", ["learned", "rotary"])
+def test_another_module_in_the_token_tables_place(pos):
+    m = _model(pos, qk_norm=False)
+    idx = torch.randint(0, 512, (2, 33))
+    want, pipe = m(idx), gpt2.EmbeddingPipe(m.cfg)
+    pipe.load_state_dict({k: v for k, v in m.state_dict().items() if k in pipe.state_dict()})
+    first = pipe(idx)
+    for module in (m, pipe):
+        plain = torch.nn.Embedding(*module.wte.weight.shape)
+        plain.load_state_dict(module.wte.state_dict())
+        module.wte = plain
+    torch.testing.assert_close(m(idx), want, rtol=0, atol=0)
+    torch.testing.assert_close(pipe(idx), first, rtol=0, atol=0)
+
+
 def _tp_parity(rank, world, d, pos):
     torch.manual_seed(0)
     cfg = gpt2.config_for("tiny", n_layer=2, n_head=4, d_model=256, vocab_size=500, max_seq_len=32, pos_emb=pos,
