@@ -48,8 +48,8 @@ class GPTConfig:
     dropout: float = 0.0
     init_std: float = 0.02
     pad_vocab_multiple: int = 128
-    qk_norm: bool = False  # RMS norm of every query and key head (one weight per feature, fp32)
     extra: Dict = field(default_factory=dict)
+    qk_norm: bool = False  # RMS norm of every query and key head (one weight per feature, fp32)
 
     @property
     def head_dim(self) -> int:

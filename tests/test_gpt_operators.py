@@ -69,6 +69,15 @@ def test_without_qk_norm_nothing_is_added():
     assert m.blocks[0].attn.q_norm.weight.dtype == torch.float32  # kept like LayerNorm's
 
 
+def test_the_configs_earlier_fields_keep_their_places():
+    from dataclasses import astuple, fields
+
+    names = [f.name for f in fields(gpt2.GPTConfig)]
+    old = [n for n in names if n != "qk_norm"]
+    cfg = gpt2.GPTConfig(*astuple(gpt2.GPTConfig(extra={"a": 1}, pad_vocab_multiple=64))[:len(old)])
+    assert old[-1] == "extra" and cfg.extra == {"a": 1} and cfg.pad_vocab_multiple == 64 and not cfg.qk_norm
+
+
 def test_token_embedding_refuses_what_its_lookup_does_not_do():
     for kw in (dict(padding_idx=0), dict(max_norm=1.0), dict(scale_grad_by_freq=True), dict(sparse=True)):
         with pytest.raises(ValueError, match="not supported"):
