@@ -108,10 +108,10 @@ class TokenEmbedding(nn.Embedding):
 
 def _embed(wte: nn.Module, wpe: Optional[nn.Embedding], idx: torch.Tensor) -> torch.Tensor:
     """Token rows, plus learned positions where there are any: in one pass, unless another module has
-    taken the token table's place (a larger vocabulary, an adapter)."""
+    taken the token table's place (a larger vocabulary, an adapter) or the tables' types differ."""
     if wpe is None:
         return wte(idx)
-    if isinstance(wte, TokenEmbedding):
+    if isinstance(wte, TokenEmbedding) and wte.weight.dtype == wpe.weight.dtype:
         return wte(idx, wpe.weight)
     return wte(idx) + wpe.weight[:idx.shape[1]].unsqueeze(0)
 

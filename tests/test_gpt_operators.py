@@ -104,6 +104,14 @@ def test_another_module_in_the_token_tables_place(pos):
     torch.testing.assert_close(pipe(idx), first, rtol=0, atol=0)
 
 
+def test_tables_of_two_types_add_in_the_wider_one():
+    pipe = gpt2.EmbeddingPipe(gpt2.config_for("tiny"))
+    pipe.wte.bfloat16()
+    idx = torch.randint(0, 512, (2, 33))
+    want = pipe.wte.weight[idx].float() + pipe.wpe.weight[:33]
+    torch.testing.assert_close(pipe(idx), want, rtol=0, atol=0)
+
+
 def _tp_parity(rank, world, d, pos):
     torch.manual_seed(0)
     cfg = gpt2.config_for("tiny", n_layer=2, n_head=4, d_model=256, vocab_size=500, max_seq_len=32, pos_emb=pos,
