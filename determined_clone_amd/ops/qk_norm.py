@@ -88,6 +88,8 @@ def _check(q, k, q_weight, k_weight, cos, sin, rot_dim, positions):
             raise ValueError(f"qk_norm_rope: positions must be [{S}] or [{B}, {S}] on {q.device}")
         positions = positions.contiguous()
     if q.is_cuda:
+        if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
+            raise ValueError("qk_norm_rope: the GPU path has no gradients for cos and sin")
         cos, sin = _f32(cos), _f32(sin)
     return cos, sin, rot, positions
 
@@ -103,7 +105,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
 
     ``q_weight`` / ``k_weight`` [D] are shared by the heads (None: no weight). ``cos`` / ``sin``
     [P, >= rot_dim / 2] are ``ops.transformer.rope_tables``; the first ``rot_dim`` features turn in
-    pairs (i, i + rot_dim / 2) (None: all of them, or none without tables). Token s uses table row s,
+    pairs (i, i + rot_dim / 2) (None: all of them, or none without tables); the tables get no
+    gradients on the GPU, which refuses ones that ask for it. Token s uses table row s,
     or ``positions`` [S] or [B, S] (int32 / int64): generation from an offset, packed documents. A
     position outside the tables raises ``IndexError`` on the CPU; the GPU path, which does not wait
     for the values, returns NaN in the rotated features (and passes NaN to that row's gradient)."""

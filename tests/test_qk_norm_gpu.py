@@ -365,3 +365,17 @@ def test_refusals():
         qk_norm_attention_qkvpacked(torch.randn(1, 2, 3, 2, 64, device="cuda"))
     with pytest.raises(RuntimeError, match="table rows"):
         _ext.load().qk_norm_rope(q, q, None, None, cos.cuda()[:1], sin.cuda()[:1], 64, None, 1e-6)
+
+
+def test_angle_tables_that_ask_for_gradients_are_refused():
+    q = torch.randn(1, 2, 2, 64, device="cuda")
+    cos, sin = T.rope_tables(2, 64, device="cuda")
+    want = qk_norm_rope(q, q, None, None, cos, sin)[0]
+    for i in range(2):
+        tables = [t.clone().requires_grad_(i == j) for j, t in enumerate((cos, sin))]
+        with pytest.raises(ValueError, match="no gradients for cos and sin"):
+            qk_norm_rope(q, q, None, None, *tables)
+        with pytest.raises(ValueError, match="no gradients for cos and sin"):
+            qk_norm_attention_qkvpacked(torch.randn(1, 2, 3, 2, 64, device="cuda").bfloat16(), None, None, *tables)
+        with torch.no_grad():
+            assert torch.equal(qk_norm_rope(q, q, None, None, *tables)[0], want)
