@@ -188,6 +188,9 @@ def qk_norm_attention_qkvpacked(qkv: torch.Tensor, q_weight: Optional[torch.Tens
     if not _attn_gpu_ok(q, k, v):
         raise ValueError("qk_norm_attention_qkvpacked: GPU path needs bf16 [B,S,3,H,D] with D in "
                          "{64,128} and 16-byte aligned rows")
+    if qkv.numel() == 0:  # no launches of nothing
+        q, k = reference_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, rot, positions, eps)
+        return reference_attention(q, k, v, causal, scale, key_lengths)
     return _QKNormAttention.apply(qkv, q_weight, k_weight, cos, sin, rot, positions, float(eps), causal,
                                   float(scale), _kv_len(key_lengths, qkv.shape[0], qkv.device))
 

@@ -379,3 +379,16 @@ def test_angle_tables_that_ask_for_gradients_are_refused():
             qk_norm_attention_qkvpacked(torch.randn(1, 2, 3, 2, 64, device="cuda").bfloat16(), None, None, *tables)
         with torch.no_grad():
             assert torch.equal(qk_norm_rope(q, q, None, None, *tables)[0], want)
+
+
+@pytest.mark.parametrize("b,s", [(0, 33), (2, 0)])
+def test_packed_attention_without_tokens(b, s):
+    """An empty output and zero weight gradients, and no failed launch left for the next call to report."""
+    qkv = torch.randn(b, s, 3, 2, 64, device="cuda").bfloat16().requires_grad_(True)
+    w = [torch.ones(64, device="cuda", requires_grad=True) for _ in range(2)]
+    cos, sin = T.rope_tables(33, 64, device="cuda")
+    out = qk_norm_attention_qkvpacked(qkv, *w, cos, sin, key_lengths=torch.ones(b, device="cuda", dtype=torch.long))
+    assert out.shape == (b, s, 2, 64) and out.dtype == torch.bfloat16
+    grads = torch.autograd.grad(out.float().sum(), [qkv] + w)
+    assert grads[0].shape == qkv.shape and not any(g.any() for g in grads)
+    assert torch.ones(5, device="cuda").sum() == 5
