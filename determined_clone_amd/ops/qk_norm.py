@@ -109,7 +109,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     gradients on the GPU, which refuses ones that ask for it. Token s uses table row s,
     or ``positions`` [S] or [B, S] (int32 / int64): generation from an offset, packed documents. A
     position outside the tables raises ``IndexError`` on the CPU; the GPU path, which does not wait
-    for the values, returns NaN in the rotated features (and passes NaN to that row's gradient)."""
+    for the values, returns NaN in the rotated features of such rows. Their gradients are NaN, and so
+    are the weights' in the rotated features, which are sums over all rows. Second derivatives raise
+    on the GPU."""
     cos, sin, rot, positions = _check(q, k, q_weight, k_weight, cos, sin, rot_dim, positions)
     if not q.is_cuda:
         return reference_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, rot, positions, eps)

@@ -392,3 +392,16 @@ def test_packed_attention_without_tokens(b, s):
     grads = torch.autograd.grad(out.float().sum(), [qkv] + w)
     assert grads[0].shape == qkv.shape and not any(g.any() for g in grads)
     assert torch.ones(5, device="cuda").sum() == 5
+
+
+def test_gradients_with_mistaken_positions():
+    """The mistake does not go unseen: NaN in its rows' gradients and in the weights' rotated features."""
+    x = [torch.randn(1, 4, 2, 64, device="cuda", requires_grad=True) for _ in range(2)]
+    w = [torch.ones(64, device="cuda", requires_grad=True) for _ in range(2)]
+    cos, sin = T.rope_tables(8, 16, device="cuda")
+    pos = torch.tensor([0, 8, 3, -1], device="cuda")
+    y = qk_norm_rope(*x, *w, cos, sin, rot_dim=16, positions=pos)
+    grads = torch.autograd.grad(y, x + w, [torch.randn(1, 4, 2, 64, device="cuda") for _ in range(2)])
+    for dx, dw in zip(grads[:2], grads[2:]):
+        assert torch.isnan(dx[0, [1, 3]]).all() and torch.isfinite(dx[0, [0, 2]]).all()
+        assert torch.isnan(dw[:16]).all() and torch.isfinite(dw[16:]).all()
