@@ -13,7 +13,8 @@ The reference's GPT-NeoX trial trains with ``model_parallel_size: 2``
 * token embedding and the tied LM head are vocab-parallel; the loss is the vocab-parallel
   cross-entropy, so the [tokens, vocab] logits are never gathered;
 * LayerNorms, position embeddings, row-parallel biases and the query / key norms' weights (whose
-  gradient is summed over the ranks' heads) are replicated (identical gradients on every TP rank; :func:`~determined_clone_amd.parallel.tensor.tp_norm_setup` counts them once).
+  gradient is summed over the ranks' heads) are replicated (identical gradients on every TP rank;
+  :func:`~determined_clone_amd.parallel.tensor.tp_norm_setup` counts them once).
 
 ``TPGPT.load_from(full)`` copies a dense model's weights into the shards (parity tests, and
 converting dense checkpoints); ``full_state_dict()`` gathers them back.

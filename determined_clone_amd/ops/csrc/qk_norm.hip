@@ -6,7 +6,7 @@
 // Backward:  g = R(p)^T dy,  dw = sum over rows of g n,  dx = r (g w - n mean(g w n)).
 //
 // Bound by HBM: 2 passes forward (x in, y out), 3 backward (x and dy in, dx out). At 32x1024 tokens,
-// 20 + 20 heads of 64 in bf16 (168 MB a pass): forward 72 us, 4.7 TB/s; backward 102 us, 4.9 TB/s; a
+// 20 + 20 heads of 64 in bf16 (168 MB a pass): forward 73 us, 4.6 TB/s; backward 102 us, 4.9 TB/s; a
 // large copy reaches 5.1 TB/s. A row takes L lanes
 // (the power of two at or above D / V), so a wave works on 64 / L heads of one token at a time and
 // walks through its q heads, then its k heads: the angles and the weights stay in registers for the
